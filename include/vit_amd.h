@@ -305,6 +305,30 @@ int va_mse_loss(const float* x, const float* y, float* loss, float* dx, float* w
 int va_gated_delta_seq(const float* q, const float* k, const float* v, const float* alpha, const float* beta,
                        const float* state_in, float* out, float* state_out, int64_t B, int64_t L, int64_t H, int64_t hd,
                        va_stream_t stream);
+
+/* The same recurrence in its chunked form (64 tokens at a time on the matrix pipe; another order of summation than
+ * va_gated_delta_seq), for whole sequences, with its gradient, and for one token:
+ *     S_t = a_t S_{t-1} (I - b_t k_t k_t^T) + b_t v_t k_t^T,   o_t = S_t q_t
+ * q, k, v: rows of token (b, t) `ld*` elements apart (a multiple of 4, at least H*hd), heads side by side, all f32 or all
+ * bf16 (is_bf16; 8-byte alignment is enough then); alpha, beta: contiguous f32 [B,L,H]; states f32 [B,H,hd,hd] (rows = value
+ * index); out / gradients of q, k, v: contiguous [B,L,H,hd] of the inputs' type.  hd 64 or 128.  Products and states are
+ * f32 whatever the type.  A non-finite token spreads over the 64-token chunk it lies in, earlier tokens included.
+ *   fwd:  state_in NULL = zeros.  workspace: va_gated_delta_fwd_workspace_floats f32 values.
+ *   bwd:  d_out, and d_state (of the final state; NULL = zeros) -> dq, dk, dv, dalpha, dbeta [, d_state_in unless NULL];
+ *         nothing is kept from the forward.  workspace: va_gated_delta_bwd_workspace_floats f32 values.
+ *   step: q, k, v [B, ld*], alpha, beta [B,H]; `state` is updated in place; out [B,H,hd]. */
+int64_t va_gated_delta_fwd_workspace_floats(int64_t B, int64_t L, int64_t H, int64_t hd);
+int64_t va_gated_delta_bwd_workspace_floats(int64_t B, int64_t L, int64_t H, int64_t hd);
+int va_gated_delta_fwd(const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv, int is_bf16,
+                       const float* alpha, const float* beta, const float* state_in, void* out, float* state_out,
+                       float* workspace, int64_t B, int64_t L, int64_t H, int64_t hd, va_stream_t stream);
+int va_gated_delta_bwd(const void* d_out, const float* d_state, const void* q, const void* k, const void* v, int64_t ldq,
+                       int64_t ldk, int64_t ldv, int is_bf16, const float* alpha, const float* beta, const float* state_in,
+                       void* dq, void* dk, void* dv, float* dalpha, float* dbeta, float* d_state_in, float* workspace,
+                       int64_t B, int64_t L, int64_t H, int64_t hd, va_stream_t stream);
+int va_gated_delta_step(const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv, int is_bf16,
+                        const float* alpha, const float* beta, float* state, void* out, int64_t B, int64_t H, int64_t hd,
+                        va_stream_t stream);
 /* Causal depthwise conv1d with 4 taps + bias + SiLU over x f32 [B, L, C] (nn.Conv1d(C, C, 4, padding=3,
  * groups=C) cut to the first L outputs, swm:452-457 / 484-486, then swm:489-491): out[b,t,c] =
  * silu(bias[c] + sum_i w[c][i] * x[b, t-3+i, c]); with normalize != 0 each row is then divided by

@@ -67,6 +67,12 @@ SIGNATURES = {
     "va_multi_sumsq": (ci, [vp, vp, i64, vp, vp, vp]),
     "va_multi_adamw": (ci, [vp, vp, i64, cf, cf, cf, cf, cf, vp, cf, vp]),
     "va_gated_delta_seq": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp]),
+    "va_gated_delta_fwd_workspace_floats": (i64, [i64, i64, i64, i64]),
+    "va_gated_delta_bwd_workspace_floats": (i64, [i64, i64, i64, i64]),
+    "va_gated_delta_fwd": (ci, [vp, vp, vp, i64, i64, i64, ci, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp]),
+    "va_gated_delta_bwd": (ci, [vp, vp, vp, vp, vp, i64, i64, i64, ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64,
+                                i64, vp]),
+    "va_gated_delta_step": (ci, [vp, vp, vp, i64, i64, i64, ci, vp, vp, vp, vp, i64, i64, i64, vp]),
     "va_dwconv1d_causal_silu": (ci, [vp, vp, vp, vp, i64, i64, i64, ci, vp]),
     "va_gate_layernorm_fwd": (ci, [vp, vp, vp, vp, vp, vp, i64, i64, cf, vp]),
     "va_dwconv1d_causal_silu_bf16": (ci, [vp, i64, vp, vp, vp, i64, i64, i64, ci, vp]),

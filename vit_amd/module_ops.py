@@ -227,3 +227,32 @@ class MlpFn(torch.autograd.Function):
         db1 = torch.zeros(hidden, dtype=F32, device=g.device)
         ops.gemm_tn_accum(d_wide, hb, dw1, dbias=db1)
         return dh, dw1, db1, dw2, db2, (g if ctx.has_resid else None), None
+
+
+class GatedDeltaFn(torch.autograd.Function):
+    """Gated delta rule over a sequence (swm:523-555) with the gradients of every input and of the carried state."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, alpha, beta, state):
+        args = [None if t is None else t.detach() for t in (q, k, v, alpha, beta, state)]
+        out, new_state = ops.gated_delta_fwd(*args)
+        ctx.save_for_backward(q, k, v, alpha, beta, state)
+        ctx.set_materialize_grads(False)
+        return out, new_state
+
+    @staticmethod
+    def backward(ctx, d_out, d_state):
+        q, k, v, alpha, beta, state = ctx.saved_tensors
+        if d_out is None and d_state is None:
+            return (None,) * 6
+        d_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if d_out is None else d_out.contiguous()
+        want = state is not None and ctx.needs_input_grad[5]
+        grads = ops.gated_delta_bwd(d_out, None if d_state is None else d_state.contiguous(), q, k, v, alpha, beta, state, want)
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad))
+
+
+def gated_delta(q, k, v, alpha, beta, state=None):
+    """Differentiable `ops.gated_delta_fwd`: (out, new state).  alpha, beta and the state are made f32 and contiguous."""
+    alpha, beta = alpha.to(F32).contiguous(), beta.to(F32).contiguous()
+    state = None if state is None else state.to(F32).contiguous()
+    return GatedDeltaFn.apply(q, k, v, alpha, beta, state)

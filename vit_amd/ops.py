@@ -443,6 +443,95 @@ def gated_delta_seq(q, k, v, alpha, beta, state=None):
     return out, new_state
 
 
+def _heads_ld(t: torch.Tensor, name: str) -> int:
+    """Elements between the token rows of q / k / v [B, L, H, hd] (or [B, H, hd]): heads lie side by side in a row, rows
+    one constant stride apart over the whole batch (a contiguous tensor, or a column block of a wider matrix)."""
+    lead, H, hd = t.shape[:-2], t.shape[-2], t.shape[-1]
+    if t.stride(-1) != 1 or (H > 1 and t.stride(-2) != hd):
+        raise ValueError(f"{name}: the heads of a token must lie side by side")
+    ld = None
+    for size, stride, rows in zip(reversed(lead), reversed(t.stride()[:-2]), ([1, lead[-1]] if len(lead) > 1 else [1])):
+        if size > 1:
+            if stride % rows or (ld is not None and stride != rows * ld):
+                raise ValueError(f"{name}: token rows must be one constant stride apart")
+            ld = stride // rows
+    return H * hd if ld is None else ld
+
+
+def _delta_operands(who: str, q, k, v, alpha, beta, state, lead: int):
+    if q.dtype not in (F32, BF16):
+        raise TypeError(f"{who}: q, k, v must be f32 or bf16")
+    if q.dim() != lead + 2:
+        raise ValueError(f"{who}: q must have {lead + 2} dimensions")
+    if 0 in q.shape:
+        raise ValueError(f"{who}: empty problem")
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        _need(x, q.dtype, name)
+        if x.shape != q.shape:
+            raise ValueError(f"{who}: q, k, v must share one shape")
+    for name, x in (("alpha", alpha), ("beta", beta)):
+        _need(x, F32, name)
+        if x.shape != q.shape[:-1] or not x.is_contiguous():
+            raise ValueError(f"{who}: {name} must be contiguous {tuple(q.shape[:-1])}")
+    B, H, hd = q.shape[0], q.shape[-2], q.shape[-1]
+    if state is not None:
+        _need(state, F32, "state")
+        if tuple(state.shape) != (B, H, hd, hd) or not state.is_contiguous():
+            raise ValueError(f"{who}: state must be contiguous [B,H,hd,hd]")
+    return _heads_ld(q, "q"), _heads_ld(k, "k"), _heads_ld(v, "v")
+
+
+def gated_delta_fwd(q, k, v, alpha, beta, state=None):
+    """The recurrence of `gated_delta_seq` in its chunked form (products over 64 tokens on the matrix pipe): q, k, v f32 or
+    bf16 [B,L,H,hd] (rows any constant stride apart), hd 64 or 128; alpha, beta f32 [B,L,H]; state f32 [B,H,hd,hd] or None
+    -> (out [B,L,H,hd] of q's type, new state f32).  A non-finite token spreads over its chunk of 64."""
+    lds = _delta_operands("gated_delta_fwd", q, k, v, alpha, beta, state, 2)
+    B, L, H, hd = q.shape
+    lib = _lib.load()
+    out = torch.empty(B, L, H, hd, dtype=q.dtype, device=q.device)
+    new_state = torch.empty(B, H, hd, hd, dtype=F32, device=q.device)
+    ws = torch.empty(lib.va_gated_delta_fwd_workspace_floats(B, L, H, hd), dtype=F32, device=q.device)
+    check(lib.va_gated_delta_fwd(_p(q), _p(k), _p(v), *lds, int(q.dtype == BF16), _p(alpha), _p(beta), _p(state), _p(out),
+                                 _p(new_state), _p(ws), B, L, H, hd, _stream()), "va_gated_delta_fwd")
+    return out, new_state
+
+
+def gated_delta_bwd(d_out, d_state, q, k, v, alpha, beta, state=None, want_state: bool = True):
+    """Gradients of `gated_delta_fwd`: d_out as out, d_state (of the final state) f32 or None -> (dq, dk, dv of q's type,
+    dalpha, dbeta f32, gradient of the initial state f32 or None).  Takes the forward's inputs; recomputes the rest."""
+    lds = _delta_operands("gated_delta_bwd", q, k, v, alpha, beta, state, 2)
+    B, L, H, hd = q.shape
+    _need(d_out, q.dtype, "d_out")
+    if d_out.shape != q.shape or not d_out.is_contiguous():
+        raise ValueError("gated_delta_bwd: d_out must be contiguous and of q's shape")
+    if d_state is not None:
+        _need(d_state, F32, "d_state")
+        if tuple(d_state.shape) != (B, H, hd, hd) or not d_state.is_contiguous():
+            raise ValueError("gated_delta_bwd: d_state must be contiguous [B,H,hd,hd]")
+    lib = _lib.load()
+    dq, dk, dv = (torch.empty(B, L, H, hd, dtype=q.dtype, device=q.device) for _ in range(3))
+    da, db = torch.empty_like(alpha), torch.empty_like(beta)
+    ds = torch.empty(B, H, hd, hd, dtype=F32, device=q.device) if want_state else None
+    ws = torch.empty(lib.va_gated_delta_bwd_workspace_floats(B, L, H, hd), dtype=F32, device=q.device)
+    check(lib.va_gated_delta_bwd(_p(d_out), _p(d_state), _p(q), _p(k), _p(v), *lds, int(q.dtype == BF16), _p(alpha), _p(beta),
+                                 _p(state), _p(dq), _p(dk), _p(dv), _p(da), _p(db), _p(ds), _p(ws), B, L, H, hd, _stream()),
+          "va_gated_delta_bwd")
+    return dq, dk, dv, da, db, ds
+
+
+def gated_delta_step_(q, k, v, alpha, beta, state):
+    """One token of every stream: q, k, v f32 or bf16 [B,H,hd] (rows any constant stride apart), alpha, beta f32 [B,H];
+    `state` f32 [B,H,hd,hd] is updated in place.  Returns out [B,H,hd] of q's type."""
+    if state is None:
+        raise ValueError("gated_delta_step_: a state to update is required")
+    lds = _delta_operands("gated_delta_step_", q, k, v, alpha, beta, state, 1)
+    B, H, hd = q.shape
+    out = torch.empty(B, H, hd, dtype=q.dtype, device=q.device)
+    check(_lib.load().va_gated_delta_step(_p(q), _p(k), _p(v), *lds, int(q.dtype == BF16), _p(alpha), _p(beta), _p(state),
+                                          _p(out), B, H, hd, _stream()), "va_gated_delta_step")
+    return out
+
+
 def dwconv1d_causal_silu(x, weight, bias, normalize: bool):
     """x f32 [B,L,C]; weight f32 [C,1,4] (nn.Conv1d layout) or [C,4]; bias [C] -> silu(causal conv) [, row-L2-normalised]."""
     _need(x, F32, "x"); _need(weight, F32, "weight"); _need(bias, F32, "bias")
