@@ -329,6 +329,29 @@ int va_gated_delta_bwd(const void* d_out, const float* d_state, const void* q, c
 int va_gated_delta_step(const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv, int is_bf16,
                         const float* alpha, const float* beta, float* state, void* out, int64_t B, int64_t H, int64_t hd,
                         va_stream_t stream);
+
+/* ---- 8-bit key/value cache and the attention over it (incremental form of va_attn_fwd_block_causal) -----------------
+ * Tokens of a stream b and head h: e4m3 codes k8, v8 [B,H,cap,hd] (cap a multiple of 64, hd 64 or 128) with one f32 scale
+ * per block of 64 tokens, k_scale, v_scale [B,H,cap/64]: the smallest power of two, 2^-100 at least, that brings the block's
+ * largest finite magnitude to 448 or below (1 for a block of zeros; infinite elements become NaN); the block that is not full
+ * yet as bf16 in k_open, v_open [B,H,64,hd].  lengths: int32 [B], tokens held.  All contiguous, on the device.
+ *   append: n tokens of every stream (of stream b only the first new_tokens[b], clamped to 0..n; NULL = n) behind its
+ *           length; k, v bf16, heads of a token side by side, tokens ld* and streams bs* elements apart (multiples of 8).
+ *           Advances lengths.  Tokens that would pass cap are dropped and the length stays at cap.
+ *   attn:   q bf16 [B,n,H*group,hd] strided like k; out bf16 contiguous.  The queries are the newest n (new_tokens[b]) tokens
+ *           of each stream, already appended: query i stands at p = lengths[b] - new_tokens[b] + i and sees all held tokens
+ *           (tokens_per_timestep 0) or those before the end of its timestep, j < (p / T + 1) T (T = 1: causal).  Rows from
+ *           new_tokens[b] on, and queries that see nothing, are zeros.  Query head h reads key/value head h / group.
+ *           max_len (<= cap): an upper bound of the lengths if the host has one; it only chooses how many pieces the keys are
+ *           split into.  workspace: va_kv8_attn_workspace_floats f32 values for the same sizes (may be 0). */
+int va_kv8_append(const void* k, const void* v, int64_t ldk, int64_t ldv, int64_t bsk, int64_t bsv, const int32_t* new_tokens,
+                  int64_t n, void* k8, void* v8, float* k_scale, float* v_scale, void* k_open, void* v_open, int32_t* lengths,
+                  int64_t B, int64_t H, int64_t hd, int64_t cap, va_stream_t stream);
+int64_t va_kv8_attn_workspace_floats(int64_t B, int64_t n, int64_t H, int64_t group, int64_t hd, int64_t max_len);
+int va_kv8_attn(const void* q, int64_t ldq, int64_t bsq, const int32_t* new_tokens, const void* k8, const void* v8,
+                const float* k_scale, const float* v_scale, const void* k_open, const void* v_open, const int32_t* lengths,
+                void* out, float* workspace, int64_t B, int64_t n, int64_t H, int64_t group, int64_t hd, int64_t cap,
+                int64_t max_len, int64_t tokens_per_timestep, float scale, va_stream_t stream);
 /* Causal depthwise conv1d with 4 taps + bias + SiLU over x f32 [B, L, C] (nn.Conv1d(C, C, 4, padding=3,
  * groups=C) cut to the first L outputs, swm:452-457 / 484-486, then swm:489-491): out[b,t,c] =
  * silu(bias[c] + sum_i w[c][i] * x[b, t-3+i, c]); with normalize != 0 each row is then divided by
@@ -352,6 +375,17 @@ int va_dwconv1d_causal_silu_bf16(const void* x_bf16, int64_t ldx, const float* w
                                  int64_t L, int64_t C, int normalize, va_stream_t stream);
 int va_gate_layernorm_fwd_g16(const float* o, const float* gate, const void* g_bf16, int64_t ldg, const float* gamma,
                               const float* beta, void* y_bf16, int64_t M, int64_t D, float eps, va_stream_t stream);
+
+/* The same stage for rows of any width (a multiple of 4, at most 4096) with its gradient: y = LayerNorm((o * gate) * silu(g));
+ * o, gate, g, y, dy and their gradients contiguous [M,D], all f32 or all bf16 (is_bf16); gamma, beta, their gradients, mean
+ * and rstd (one per row, both NULL for a forward that keeps nothing) f32.  The gradient overwrites all its outputs; workspace:
+ * va_gated_layernorm_bwd_workspace_floats f32 values. */
+int va_gated_layernorm_fwd(const void* o, const void* gate, const void* g, int is_bf16, const float* gamma, const float* beta,
+                           void* y, float* mean, float* rstd, int64_t M, int64_t D, float eps, va_stream_t stream);
+int64_t va_gated_layernorm_bwd_workspace_floats(int64_t M, int64_t D);
+int va_gated_layernorm_bwd(const void* dy, const void* o, const void* gate, const void* g, int is_bf16, const float* gamma,
+                           const float* mean, const float* rstd, void* d_o, void* d_gate, void* d_g, float* dgamma,
+                           float* dbeta, float* workspace, int64_t M, int64_t D, va_stream_t stream);
 
 /* The layer's two per-head gates, alpha = sigmoid(x @ wa^T) and beta = sigmoid(x @ wb^T) (swm:448-449, 494-495; the
  * projections have no bias): x f32 [M, D] contiguous, D = 1024; wa, wb f32 [H, D], H <= 8; alpha, beta f32 [M, H].

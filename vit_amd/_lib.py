@@ -73,6 +73,9 @@ SIGNATURES = {
     "va_gated_delta_bwd": (ci, [vp, vp, vp, vp, vp, i64, i64, i64, ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64,
                                 i64, vp]),
     "va_gated_delta_step": (ci, [vp, vp, vp, i64, i64, i64, ci, vp, vp, vp, vp, i64, i64, i64, vp]),
+    "va_kv8_append": (ci, [vp, vp, i64, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp]),
+    "va_kv8_attn_workspace_floats": (i64, [i64, i64, i64, i64, i64, i64]),
+    "va_kv8_attn": (ci, [vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, cf, vp]),
     "va_dwconv1d_causal_silu": (ci, [vp, vp, vp, vp, i64, i64, i64, ci, vp]),
     "va_gate_layernorm_fwd": (ci, [vp, vp, vp, vp, vp, vp, i64, i64, cf, vp]),
     "va_dwconv1d_causal_silu_bf16": (ci, [vp, i64, vp, vp, vp, i64, i64, i64, ci, vp]),
@@ -85,6 +88,9 @@ SIGNATURES = {
     "va_mse_workspace_floats": (i64, [i64]),
     "va_mse_loss": (ci, [vp, vp, vp, vp, vp, i64, cf, vp]),
     "va_delta_gates_fwd": (ci, [vp, vp, vp, vp, vp, vp, i64, i64, i64, vp]),
+    "va_gated_layernorm_fwd": (ci, [vp, vp, vp, ci, vp, vp, vp, vp, vp, i64, i64, cf, vp]),
+    "va_gated_layernorm_bwd_workspace_floats": (i64, [i64, i64]),
+    "va_gated_layernorm_bwd": (ci, [vp, vp, vp, vp, ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, vp]),
     "va_gate_layernorm_fwd_g16": (ci, [vp, vp, vp, i64, vp, vp, vp, i64, i64, cf, vp]),
 }
 

@@ -256,3 +256,30 @@ def gated_delta(q, k, v, alpha, beta, state=None):
     alpha, beta = alpha.to(F32).contiguous(), beta.to(F32).contiguous()
     state = None if state is None else state.to(F32).contiguous()
     return GatedDeltaFn.apply(q, k, v, alpha, beta, state)
+
+
+class GatedLayerNormFn(torch.autograd.Function):
+    """LayerNorm((o * gate) * silu(g)), the memory layer's output stage (swm:511-519), with all its gradients."""
+
+    @staticmethod
+    def forward(ctx, o, gate, g, gamma, beta, eps):
+        shape = o.shape
+        rows = [t.detach().reshape(-1, shape[-1]).contiguous() for t in (o, gate, g)]
+        gamma = gamma.detach()
+        y, mean, rstd = ops.gated_layernorm_fwd(*rows, gamma, beta.detach(), eps, keep=any(ctx.needs_input_grad))
+        if mean is not None:
+            ctx.save_for_backward(*rows, gamma, mean, rstd)
+        return y.view(shape)
+
+    @staticmethod
+    def backward(ctx, dy):
+        rows, (gamma, mean, rstd) = ctx.saved_tensors[:3], ctx.saved_tensors[3:]
+        shape = dy.shape
+        grads = ops.gated_layernorm_bwd(dy.reshape(rows[0].shape).contiguous(), *rows, gamma, mean, rstd)
+        grads = [x.view(shape) for x in grads[:3]] + list(grads[3:])
+        return tuple(x if need else None for x, need in zip(grads, ctx.needs_input_grad)) + (None,)
+
+
+def gated_layernorm(o, gate, g, gamma, beta, eps: float = 1e-5):
+    """Differentiable `ops.gated_layernorm_fwd` over the last dimension; o, gate, g of one shape and type (f32 or bf16)."""
+    return GatedLayerNormFn.apply(o, gate, g, gamma, beta, float(eps))

@@ -405,6 +405,112 @@ def attn_bwd(qkv, out, d_out, lse2, dqkv, B: int, N: int, H: int, drop_key: int 
     return dqkv
 
 
+KV8_BLOCK = 64          # tokens that share one scale
+
+
+class KVCache8:
+    """Keys and values of `lengths` tokens per stream in 8 bits: e4m3 codes k8, v8 [B, H, capacity, hd] with one f32
+    power-of-two scale per block of 64 tokens and head (k_scale, v_scale [B, H, capacity / 64]); the block that is not full yet
+    lies in k_open, v_open [B, H, 64, hd] bf16.  A code times its scale is the value it stands for.  `max_len` is the host's
+    upper bound of the lengths (they live on the device): `kv8_append_` raises when it would pass the capacity."""
+
+    def __init__(self, k8, v8, k_scale, v_scale, k_open, v_open, lengths, max_len: Optional[int] = None):
+        if k8.dim() != 4 or k8.shape[2] % KV8_BLOCK or 0 in k8.shape:
+            raise ValueError("KVCache8: k8 must be [B, H, capacity, hd], the capacity a multiple of 64")
+        B, H, cap, hd = k8.shape
+        for name, t, dtype, shape in (("k8", k8, torch.float8_e4m3fn, (B, H, cap, hd)), ("v8", v8, torch.float8_e4m3fn, (B, H, cap, hd)),
+                                      ("k_scale", k_scale, F32, (B, H, cap // KV8_BLOCK)),
+                                      ("v_scale", v_scale, F32, (B, H, cap // KV8_BLOCK)),
+                                      ("k_open", k_open, BF16, (B, H, KV8_BLOCK, hd)), ("v_open", v_open, BF16, (B, H, KV8_BLOCK, hd)),
+                                      ("lengths", lengths, torch.int32, (B,))):
+            _need(t, dtype, name)
+            if t.shape != shape or not t.is_contiguous():
+                raise ValueError(f"KVCache8: {name} must be contiguous {shape}")
+        if max_len is not None and not 0 <= max_len <= cap:
+            raise ValueError("KVCache8: max_len must lie between 0 and the capacity")
+        self.k8, self.v8, self.k_scale, self.v_scale = k8, v8, k_scale, v_scale
+        self.k_open, self.v_open, self.lengths = k_open, v_open, lengths
+        self.batch, self.heads, self.capacity, self.head_dim = B, H, cap, hd
+        self.max_len = cap if max_len is None else int(max_len)
+
+    @classmethod
+    def empty(cls, batch: int, heads: int, head_dim: int, capacity: int, device) -> "KVCache8":
+        """A cache with no tokens; the capacity is rounded up to whole blocks."""
+        blocks = -(-capacity // KV8_BLOCK)
+        new = lambda dtype, *shape: torch.zeros(batch, heads, *shape, dtype=dtype, device=device)      # noqa: E731
+        codes = [new(torch.uint8, blocks * KV8_BLOCK, head_dim).view(torch.float8_e4m3fn) for _ in range(2)]
+        scales = [new(F32, blocks).fill_(1.0) for _ in range(2)]
+        opened = [new(BF16, KV8_BLOCK, head_dim) for _ in range(2)]
+        return cls(*codes, *scales, *opened, torch.zeros(batch, dtype=torch.int32, device=device), max_len=0)
+
+    def reset(self) -> None:
+        """Forget all tokens."""
+        self.lengths.zero_()
+        self.max_len = 0
+
+
+def _token_strides(t: torch.Tensor, name: str, shape) -> Tuple[int, int]:
+    """(elements between tokens, between streams) of bf16 [B, n, heads, hd] with the heads of a token side by side."""
+    _need(t, BF16, name)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.stride(3) != 1 or (t.shape[2] > 1 and t.stride(2) != t.shape[3]):
+        raise ValueError(f"{name}: the heads of a token must lie side by side")
+    return (t.stride(1) if t.shape[1] > 1 else t.shape[2] * t.shape[3]), (t.stride(0) if t.shape[0] > 1 else 0)
+
+
+def _new_tokens(new: Optional[torch.Tensor], B: int):
+    if new is not None:
+        _need(new, torch.int32, "new")
+        if tuple(new.shape) != (B,) or not new.is_contiguous():
+            raise ValueError("new must be a contiguous int32 [B] tensor")
+
+
+def kv8_append_(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, new: Optional[torch.Tensor] = None) -> KVCache8:
+    """Put k, v bf16 [B, n, H, hd] (any token and stream strides) behind the streams' tokens; of stream b only the first
+    new[b] (int32 [B] on the device; None: all n).  A block is quantised when its 64 tokens are there, so the codes do not
+    depend on how many tokens came per call."""
+    B, H, hd = cache.batch, cache.heads, cache.head_dim
+    if k.dim() != 4 or k.shape[1] == 0:
+        raise ValueError("kv8_append_: k must be [B, n, H, hd] with at least one token")
+    n = k.shape[1]
+    ldk, bsk = _token_strides(k, "k", (B, n, H, hd))
+    ldv, bsv = _token_strides(v, "v", (B, n, H, hd))
+    _new_tokens(new, B)
+    if cache.max_len + n > cache.capacity:
+        raise ValueError(f"kv8_append_: {n} tokens behind up to {cache.max_len} pass the capacity of {cache.capacity}")
+    check(_lib.load().va_kv8_append(_p(k), _p(v), ldk, ldv, bsk, bsv, _p(new), n, _p(cache.k8), _p(cache.v8), _p(cache.k_scale),
+                                    _p(cache.v_scale), _p(cache.k_open), _p(cache.v_open), _p(cache.lengths), B, H, hd,
+                                    cache.capacity, _stream()), "va_kv8_append")
+    cache.max_len += n
+    return cache
+
+
+def kv8_attn(q: torch.Tensor, cache: KVCache8, new: Optional[torch.Tensor] = None, tokens_per_timestep: int = 0,
+             scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of the streams' newest tokens (already appended) over the cache: q bf16 [B, n, heads, hd], heads a multiple of
+    the cache's (consecutive query heads share a key/value head); of stream b the first new[b] rows (None: all n) are its
+    last tokens, the others give zeros.  tokens_per_timestep 0: every query sees all tokens held; T > 0: those before the end
+    of its own timestep of T tokens (1: causal).  scale: 1/sqrt(hd) by default.  Returns bf16 [B, n, heads, hd]."""
+    B, H, hd = cache.batch, cache.heads, cache.head_dim
+    if q.dim() != 4 or q.shape[1] == 0 or q.shape[2] == 0 or q.shape[2] % H:
+        raise ValueError("kv8_attn: q must be [B, n, heads, hd] with heads a multiple of the cache's")
+    n, Hq = q.shape[1], q.shape[2]
+    ldq, bsq = _token_strides(q, "q", (B, n, Hq, hd))
+    _new_tokens(new, B)
+    if tokens_per_timestep < 0:
+        raise ValueError("kv8_attn: tokens_per_timestep must not be negative")
+    lib = _lib.load()
+    out = torch.empty(B, n, Hq, hd, dtype=BF16, device=q.device)
+    floats = lib.va_kv8_attn_workspace_floats(B, n, H, Hq // H, hd, cache.max_len)
+    ws = torch.empty(floats, dtype=F32, device=q.device) if floats else None
+    check(lib.va_kv8_attn(_p(q), ldq, bsq, _p(new), _p(cache.k8), _p(cache.v8), _p(cache.k_scale), _p(cache.v_scale),
+                          _p(cache.k_open), _p(cache.v_open), _p(cache.lengths), _p(out), _p(ws), B, n, H, Hq // H, hd,
+                          cache.capacity, cache.max_len, tokens_per_timestep, hd ** -0.5 if scale is None else float(scale),
+                          _stream()), "va_kv8_attn")
+    return out
+
+
 def dropout(x: torch.Tensor, key: int, p: float, out: Optional[torch.Tensor] = None,
             resid: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out = [resid +] keep(x) / (1 - p) with the counter-based masks of the library (training-mode nn.Dropout,
@@ -568,6 +674,53 @@ def gate_layernorm_fwd(o, gate, g, gamma, beta, out, eps: float = 1e-5):
     check(_lib.load().va_gate_layernorm_fwd(_p(o), _p(gate), _p(g), _p(gamma), _p(beta), _p(out), M, D, eps, _stream()),
           "va_gate_layernorm_fwd")
     return out
+
+
+def _gated_norm_operands(who: str, gamma, *rows):
+    x = rows[0][1]
+    if x.dtype not in (F32, BF16):
+        raise TypeError(f"{who}: tensors must be f32 or bf16")
+    if x.dim() != 2 or 0 in x.shape:
+        raise ValueError(f"{who}: o must be a non-empty [M, D] matrix")
+    for name, t in rows:
+        _need(t, x.dtype, name)
+        if t.shape != x.shape or not t.is_contiguous():
+            raise ValueError(f"{who}: {name} must be contiguous and of o's shape")
+    for name, t in gamma:
+        _need(t, F32, name)
+        if t.numel() != x.shape[1] or not t.is_contiguous():
+            raise ValueError(f"{who}: {name} must be a contiguous [D] vector")
+
+
+def gated_layernorm_fwd(o, gate, g, gamma, beta, eps: float = 1e-5, keep: bool = True):
+    """y = LayerNorm((o * gate) * silu(g)) over rows of any width (a multiple of 4, at most 4096): o, gate, g contiguous
+    [M, D], all f32 or all bf16; gamma, beta f32 [D] -> (y of o's type, mean, rstd f32 [M] or None, None with keep=False)
+    (swm:511-519)."""
+    _gated_norm_operands("gated_layernorm_fwd", (("gamma", gamma), ("beta", beta)), ("o", o), ("gate", gate), ("g", g))
+    M, D = o.shape
+    y = torch.empty_like(o)
+    mean, rstd = (torch.empty(M, dtype=F32, device=o.device) if keep else None for _ in range(2))
+    check(_lib.load().va_gated_layernorm_fwd(_p(o), _p(gate), _p(g), int(o.dtype == BF16), _p(gamma), _p(beta), _p(y), _p(mean),
+                                             _p(rstd), M, D, float(eps), _stream()), "va_gated_layernorm_fwd")
+    return y, mean, rstd
+
+
+def gated_layernorm_bwd(dy, o, gate, g, gamma, mean, rstd):
+    """Gradients of `gated_layernorm_fwd`: (d_o, d_gate, d_g of o's type, dgamma, dbeta f32)."""
+    _gated_norm_operands("gated_layernorm_bwd", (("gamma", gamma),), ("o", o), ("gate", gate), ("g", g), ("dy", dy))
+    M, D = o.shape
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        _need(t, F32, name)
+        if t.numel() != M or not t.is_contiguous():
+            raise ValueError(f"gated_layernorm_bwd: {name} must be a contiguous [M] vector")
+    lib = _lib.load()
+    d_o, d_gate, d_g = (torch.empty_like(o) for _ in range(3))
+    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
+    ws = torch.empty(lib.va_gated_layernorm_bwd_workspace_floats(M, D), dtype=F32, device=o.device)
+    check(lib.va_gated_layernorm_bwd(_p(dy), _p(o), _p(gate), _p(g), int(o.dtype == BF16), _p(gamma), _p(mean), _p(rstd), _p(d_o),
+                                     _p(d_gate), _p(d_g), _p(dgamma), _p(dbeta), _p(ws), M, D, _stream()),
+          "va_gated_layernorm_bwd")
+    return d_o, d_gate, d_g, dgamma, dbeta
 
 
 # ------------------------------------------------------------------ loss heads (value and gradient per call)
