@@ -5,6 +5,9 @@ gating + LayerNorm, o-proj GEMM (+residual)] -> LayerNorm -> fc1 (+bias, GELU) -
 
 Same numeric scheme as the encoder: f32 residual stream and statistics, bf16 GEMM/attention operands with f32
 accumulation; the two 8-wide gate projections (a_proj, b_proj) are f32 dot products.
+
+`block_stream` is the same block for the newest tokens of running streams: the attention reads an 8-bit cache of all earlier
+keys and values, the recurrence and the convolutions continue from their kept state.
 """
 from __future__ import annotations
 
@@ -95,6 +98,98 @@ def block_forward(blk, x: torch.Tensor, tokens_per_timestep: int, state: Optiona
     x_out = new(D, F32)
     ops.gemm_nt(act, wc.fwd("fc2", blk.mlp[2].weight), ops.EPI_F32, x_out, bias=blk.mlp[2].bias.detach(), resid=x_mid)
     return x_out.view(B, L, D), new_state
+
+
+class BlockStream:
+    """What one predictor block keeps of `batch` streams between calls of `block_stream`: keys and values in 8 bits
+    (`ops.KVCache8`), the recurrence's state and the last three inputs of the causal convolutions."""
+
+    def __init__(self, blk, batch: int, capacity: int, device):
+        H, D = blk.spatial_attn.num_heads, blk.spatial_attn.embed_dim
+        self.kv = ops.KVCache8.empty(batch, H, D // H, capacity, device)
+        self.state = self.conv = None
+        if blk.use_deltanet:
+            t = blk.temporal_layer
+            self.state = torch.zeros(batch, t.num_heads, t.head_dim, t.head_dim, dtype=F32, device=device)
+            self.conv = torch.zeros(batch, 3, 4 * t.num_heads * t.head_dim, dtype=BF16, device=device)
+
+    def reset(self) -> None:
+        """Forget all tokens."""
+        self.kv.reset()
+        if self.state is not None:
+            self.state.zero_()
+            self.conv.zero_()
+
+
+def _memory_stream(t, x_mid: torch.Tensor, B: int, n: int, stream: BlockStream, wc: WeightCache) -> torch.Tensor:
+    """The memory layer's share of `block_stream`: x_mid f32 [B*n, D] -> the residual stream behind the layer."""
+    M, D = x_mid.shape
+    dev = x_mid.device
+    Hd, Dh = t.num_heads, t.head_dim
+    inner = Hd * Dh
+    xb = torch.empty(M, D, dtype=BF16, device=dev)
+    alpha, beta = ops.delta_gates_fwd(x_mid, t.a_proj.weight.detach(), t.b_proj.weight.detach(), xb)
+    proj = torch.empty(M, 5 * inner, dtype=BF16, device=dev)
+    ops.gemm_nt(xb, wc.fwd_cat("qkvg_proj", (t.q_proj.weight, t.k_proj.weight, t.v_proj.weight, t.g_proj.weight)), ops.EPI_BF16, proj)
+    # three earlier inputs in front of every stream's new ones (zeros before the first token: the convolution's own padding)
+    rows = n + 3
+    ext = torch.cat([stream.conv, proj.view(B, n, 5 * inner)[..., :4 * inner]], dim=1)
+    stream.conv.copy_(ext[:, n:])
+    ext = ext.view(B * rows, 4 * inner)
+    conv_w, conv_b = t.v_conv1d.weight.detach().reshape(2 * inner, 4), t.v_conv1d.bias.detach()
+
+    def conv(i, w, b, norm):
+        return ops.dwconv1d_causal_silu_bf16(ext[:, i * inner:(i + 1) * inner], B, rows, w, b, norm).view(B, rows, Hd, Dh)
+
+    q = conv(0, t.q_conv1d.weight.detach(), t.q_conv1d.bias.detach(), True)
+    k = conv(1, t.k_conv1d.weight.detach(), t.k_conv1d.bias.detach(), True)
+    v = conv(2, conv_w[:inner], conv_b[:inner], False)
+    gate = conv(3, conv_w[inner:], conv_b[inner:], False)
+    if n == 1:
+        out = ops.gated_delta_step_(q[:, 3], k[:, 3], v[:, 3], alpha, beta, stream.state)
+    else:
+        # the three leading rows leave the state as it is: decay 1, nothing written
+        a_ext = torch.cat([alpha.new_ones(B, 3, Hd), alpha.view(B, n, Hd)], dim=1)
+        b_ext = torch.cat([beta.new_zeros(B, 3, Hd), beta.view(B, n, Hd)], dim=1)
+        out, state = ops.gated_delta_fwd(q, k, v, a_ext, b_ext, stream.state)
+        stream.state.copy_(state)
+        out = out[:, 3:]
+    on = torch.empty(M, inner, dtype=BF16, device=dev)
+    out, gate = (z.reshape(M, inner).contiguous() for z in (out, gate[:, 3:]))
+    ops.gate_layernorm_fwd(out, gate, proj[:, 4 * inner:], t.o_norm.weight.detach(), t.o_norm.bias.detach(), on, t.o_norm.eps)
+    x_out = torch.empty(M, D, dtype=F32, device=dev)
+    return ops.gemm_nt(on, wc.fwd("o_proj", t.o_proj.weight), ops.EPI_F32, x_out, resid=x_mid)
+
+
+def block_stream(blk, x: torch.Tensor, stream: BlockStream, tokens_per_timestep: int, wc: WeightCache) -> torch.Tensor:
+    """`block_forward` for the next tokens x f32 [B, n, D] of every stream: attention over the 8-bit cache of all tokens so
+    far, the recurrence from its state.  Updates `stream`; returns x_out [B, n, D]."""
+    B, n, D = x.shape
+    if B != stream.kv.batch:
+        raise ValueError(f"block_stream: {B} streams given, the state holds {stream.kv.batch}")
+    if n == 0 or (tokens_per_timestep > 0 and n % tokens_per_timestep):
+        raise ValueError("block_stream: whole timesteps are expected")
+    M, dev = B * n, x.device
+    a = blk.spatial_attn
+    H = a.num_heads
+    x2 = x.detach().reshape(M, D).contiguous()
+    ln = torch.empty(M, D, dtype=BF16, device=dev)
+    ops.layernorm_fwd(x2, blk.norm1.weight, blk.norm1.bias, ln, eps=blk.norm1.eps)
+    qkv = torch.empty(M, 3 * D, dtype=BF16, device=dev)
+    ops.gemm_nt(ln, wc.fwd("in_proj", a.in_proj_weight), ops.EPI_BF16, qkv, bias=a.in_proj_bias.detach())
+    q, k, v = (qkv.view(B, n, 3 * D)[..., i * D:(i + 1) * D].unflatten(-1, (H, D // H)) for i in range(3))
+    ops.kv8_append_(stream.kv, k, v)
+    attn = ops.kv8_attn(q, stream.kv, tokens_per_timestep=tokens_per_timestep).view(M, D)
+    x_mid = torch.empty(M, D, dtype=F32, device=dev)
+    ops.gemm_nt(attn, wc.fwd("out_proj", a.out_proj.weight), ops.EPI_F32, x_mid, bias=a.out_proj.bias.detach(), resid=x2)
+    if blk.use_deltanet:
+        x_mid = _memory_stream(blk.temporal_layer, x_mid, B, n, stream, wc)
+    ops.layernorm_fwd(x_mid, blk.norm2.weight, blk.norm2.bias, ln, eps=blk.norm2.eps)
+    act = torch.empty(M, 4 * D, dtype=BF16, device=dev)
+    ops.gemm_nt(ln, wc.fwd("fc1", blk.mlp[0].weight), ops.EPI_GELU_ONLY, act, bias=blk.mlp[0].bias.detach())
+    x_out = torch.empty(M, D, dtype=F32, device=dev)
+    ops.gemm_nt(act, wc.fwd("fc2", blk.mlp[2].weight), ops.EPI_F32, x_out, bias=blk.mlp[2].bias.detach(), resid=x_mid)
+    return x_out.view(B, n, D)
 
 
 def linear(x2: torch.Tensor, lin, wc: WeightCache, name: str, gelu: bool = False) -> torch.Tensor:

@@ -7,8 +7,9 @@ HIP kernels of libvit_amd.so through `vit_amd.encoder_engine` instead of eager t
 
 The encoder's building blocks (`TubeletEmbedding`, `RoPEMultiheadAttention`, `VideoViTBlock`) also run on
 their own, forward and backward, through the same kernels (`vit_amd.module_ops`).  The action-conditioned
-predictor runs its inference path (no autograd graph) on the kernels of `vit_amd.predictor_engine`; with autograd
-it uses a torch formulation of the same arithmetic.  Nothing on the encoder side has a CPU path: CPU tensors raise.
+predictor runs its inference path (no autograd graph) on the kernels of `vit_amd.predictor_engine`, a whole sequence at a
+time or token streams from a cache (`stream`, `predict_stream`); with autograd it uses a torch formulation of the same
+arithmetic around the differentiable kernels of the memory layer.  Nothing on the encoder side has a CPU path: CPU tensors raise.
 
 Reference citations: swm = surgical_world_model.py of HananKibria/VIT.
 """
@@ -416,14 +417,15 @@ def _note_torch_path(x: torch.Tensor, who: str) -> None:
     _warned_torch_path = True
     import warnings
     warnings.warn(f"{who}: grad mode is on and the predictor has trainable parameters (or its input requires grad), so "
-                  "this call is computed by the torch formulation (a per-token Python loop for the memory layer), not "
-                  "by the HIP kernels. For inference wrap the call in torch.no_grad(); the kernels have no predictor "
-                  "backward.", RuntimeWarning, stacklevel=3)
+                  "this call is computed by the torch formulation, with the memory layer's recurrence and output stage on "
+                  "their differentiable HIP kernels (head dims 64 and 128). For inference wrap the call in "
+                  "torch.no_grad().", RuntimeWarning, stacklevel=3)
 
 
 class GatedDeltaLayer(nn.Module):
-    """Gated delta-rule memory layer (swm:431-555).  Only the sequential recurrence is provided: it is the
-    form inference uses and the one the reference's other ("parallel") path fails to reproduce."""
+    """Gated delta-rule memory layer (swm:431-555).  What is computed is the sequential recurrence: the form inference uses
+    and the one the reference's other ("parallel") path fails to reproduce.  Without a graph it runs token by token in one
+    kernel; with one (f32 on the device, head dim 64 or 128) chunk by chunk, differentiable in every input and the state."""
 
     def __init__(self, hidden_size, num_heads=4, head_dim=128, chunk_size=64):
         super().__init__()
@@ -481,8 +483,18 @@ class GatedDeltaLayer(nn.Module):
             k = F.normalize(self.silu(self._causal_conv(self.k_conv1d, self.k_proj(x))), p=2, dim=-1)
             v = self.silu(self._causal_conv(self.v_conv1d, self.v_proj(x)))
             v, v_gate = v.chunk(2, dim=-1)
-            out, new_state = self._sequential_gated_delta(q.view(B, L, H, Dh), k.view(B, L, H, Dh), v.view(B, L, H, Dh),
-                                                          alpha, beta, state)
+            if x.is_cuda and q.dtype == torch.float32 and Dh in (64, 128):
+                with torch.cuda.device(x.device):
+                    # the convolutions leave (batch, channel, time) order behind
+                    out, new_state = module_ops.gated_delta(*(t.contiguous().view(B, L, H, Dh) for t in (q, k, v)), alpha, beta,
+                                                            state)
+                    if H * Dh <= 4096:
+                        out = module_ops.gated_layernorm(out.view(B, L, H * Dh), v_gate, self.g_proj(x), self.o_norm.weight,
+                                                         self.o_norm.bias, self.o_norm.eps)
+                        return self.o_proj(out), new_state
+            else:
+                out, new_state = self._sequential_gated_delta(q.view(B, L, H, Dh), k.view(B, L, H, Dh), v.view(B, L, H, Dh),
+                                                              alpha, beta, state)
         out = (out * v_gate.view(B, L, H, Dh)).reshape(B, L, -1) * self.silu(self.g_proj(x))
         return self.o_proj(self.o_norm(out)), new_state
 
@@ -571,6 +583,22 @@ class HybridPredictorBlock(nn.Module):
             delta, state = self.temporal_layer(x, state)
             x = x + delta
         return x + self.mlp(self.norm2(x)), state
+
+    def new_stream(self, batch: int, capacity: int, device) -> predictor_engine.BlockStream:
+        """State of `batch` token streams of up to `capacity` tokens each, for `stream`."""
+        return predictor_engine.BlockStream(self, batch, capacity, device)
+
+    def stream(self, x, stream, tokens_per_timestep=0):
+        """The next tokens x [B, n, D] (f32, on the device, no graph) of every stream: what `forward` with the block-causal mask
+        of `tokens_per_timestep` gives for them behind all earlier ones, from the stream's 8-bit keys and values, recurrence
+        state and convolution inputs.  n: whole timesteps (tokens_per_timestep 0: any number, each call sees all tokens so
+        far and its own)."""
+        if not _hip_inference(x, self):
+            raise VitAmdError("HybridPredictorBlock.stream: f32 tokens on a HIP device and no autograd graph are needed (wrap "
+                              "the call in torch.no_grad())")
+        if not predictor_engine.block_supported(self, x):
+            raise VitAmdError("HybridPredictorBlock.stream: the kernels take a width of 1024 with heads of 64 or 128")
+        return predictor_engine.block_stream(self, x, stream, tokens_per_timestep, _own_cache(self))
 
 
 class BlockCausalMask:
@@ -748,6 +776,21 @@ class SurgicalActionConditionedWorldModel(nn.Module):
         [patches, action, state] (swm:1428-1438)."""
         B, T, n, D = video_features.shape
         return torch.cat([video_features, action_emb[:, :, None], state_emb[:, :, None]], dim=2).reshape(B, T * (n + 2), D)
+
+    def new_predictor_streams(self, batch: int, max_timesteps: int, device):
+        """States for `predict_stream`: one per predictor block, for `batch` streams of up to `max_timesteps` timesteps."""
+        capacity = max_timesteps * (self.tokens_per_frame + 2)
+        return [blk.new_stream(batch, capacity, device) for blk in self.predictor_blocks]
+
+    @torch.no_grad()
+    def predict_stream(self, tokens, streams):
+        """The next timestep(s) of every stream through the predictor: tokens (B, T*(n+2), D) as `interleave_tokens` gives
+        them -> the normalised predictor features of those tokens, as `forward` computes them for the whole sequence so
+        far.  Each timestep costs its own tokens and one pass over the 8-bit cache instead of the whole sequence."""
+        per_step = self.tokens_per_frame + 2
+        for blk, stream in zip(self.predictor_blocks, streams, strict=True):
+            tokens = blk.stream(tokens, stream, per_step)
+        return self.predictor_norm(tokens)
 
     def forward(self, video, actions, states, predict_horizon=1, encoder_frozen=True):
         B = video.shape[0]
