@@ -21,17 +21,27 @@
 // products, never differences of logarithms).  delta_scan_kernel runs once more for U and the chunks' states, then
 // delta_rscan_kernel backwards, then delta_grad_kernel per chunk.
 //
-// All products run on the f32 matrix instruction (16x16x4): its operand for contraction index 4g+r of lane group g is
-// register r of an accumulator tile, so results (V - K M, U, M, G) feed the next product from where they lie, and a
-// left operand is one 16-byte read of a row.
+// Numbers on the matrix pipe.  The bf16 instruction (16x16x32) does sixteen times the products of the f32 one (16x16x4) per
+// cycle, so the scans split every f32 operand into three bf16 numbers, x = x0 + x1 + x2 with |x1| <= 2^-8 |x| and
+// |x2| <= 2^-16 |x| (nothing is left of 24 bits), and add the six products x_a y_b with a + b <= 2 into one f32 accumulator;
+// what is left out is below 2^-24 of |x y|, the rounding of an f32 product.  bf16 inputs are one such number: three products.
+// Where a result is rounded to bf16 in the end, two numbers per operand are kept (2^-16).  The 64x64 systems (prep) and the
+// last gradients (grad) run on the f32 instruction.
+// Both instructions take a right operand from an accumulator as it lies: register r of lane group g holds row 4g+r of a tile,
+// and any order of the contraction index will do if the left operand follows it: for the f32 one index 4g+r at step r, for
+// the bf16 one elements 0..3 from the first and 4..7 from the second of two tiles.  V - K M, U, M and G feed the next product
+// from their registers.
 #include "common.h"
 
 namespace {
 
 constexpr int DC = 64;                    // tokens per chunk
 constexpr int TRI = 10;                   // 16x16 blocks of a lower triangle of 64x64
-constexpr int FRAG = 256;                 // floats of one 16x16 operand block: lane l holds row l%16, columns 4(l/16)..+3
 constexpr int SQ = DC + 4;                // row stride of 64x64 matrices in LDS
+constexpr int BLK = 6;                    // 16x32 operand blocks that cover a triangle of 64x64
+constexpr int BFRAG = 512;                // bf16 numbers of one: lane l holds row l%16, columns 4(l/16)+{0..3, 16..19}
+
+template <int V> struct int_c { static constexpr int value = V; };
 
 VA_DEVINL f32x4_t mfma_f32(float a, float b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 // index of block (it, jt), it >= jt, of a lower triangle
@@ -42,133 +52,231 @@ VA_DEVINL f32x4_t widen4(u32x2_t p) {
     return (f32x4_t){__uint_as_float(p[0] << 16), __uint_as_float(p[0] & 0xffff0000u), __uint_as_float(p[1] << 16),
                      __uint_as_float(p[1] & 0xffff0000u)};
 }
-template <typename T> struct elem;
-template <> struct elem<float> {
+// A chunk's rows of one head through a buffer descriptor that ends behind the chunk's last token: offsets of 32 bits, rows
+// behind the sequence read as zeros and are not written, without a branch.
+template <typename T> struct ChunkOf;
+struct ChunkBase {
+    __amdgpu_buffer_rsrc_t r;
+    int row;                                      // bytes between rows
+};
+VA_DEVINL ChunkBase chunk_base(const void* first, int64_t row_bytes, int rows) {
+    ChunkBase c;
+    c.row = (int)row_bytes;
+    c.r = __builtin_amdgcn_make_buffer_rsrc((void*)first, (short)0, (int)(row_bytes * rows), 0x00020000);
+    return c;
+}
+template <> struct ChunkOf<float> {
     typedef f32x4_t raw4;
-    static VA_DEVINL float get(const float* p) { return *p; }
-    static VA_DEVINL void put(float* p, float x) { *p = x; }
+    ChunkBase c;
+    VA_DEVINL raw4 raw(int row, int col) const { return __builtin_bit_cast(raw4, __builtin_amdgcn_raw_buffer_load_b128(c.r, row * c.row + col * 4, 0, 0)); }
+    VA_DEVINL float get(int row, int col) const { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(c.r, row * c.row + col * 4, 0, 0)); }
+    VA_DEVINL void put(int row, int col, float x) const { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), c.r, row * c.row + col * 4, 0, 0); }
 };
-template <> struct elem<bf16_t> {
+template <> struct ChunkOf<bf16_t> {
     typedef u32x2_t raw4;
-    static VA_DEVINL float get(const bf16_t* p) { return bf16_to_f32(*p); }
-    static VA_DEVINL void put(bf16_t* p, float x) { *p = f32_to_bf16(x); }      // the output's own type: one rounding
+    ChunkBase c;
+    VA_DEVINL raw4 raw(int row, int col) const { return __builtin_bit_cast(raw4, __builtin_amdgcn_raw_buffer_load_b64(c.r, row * c.row + col * 2, 0, 0)); }
+    VA_DEVINL float get(int row, int col) const { return bf16_to_f32(__builtin_amdgcn_raw_buffer_load_b16(c.r, row * c.row + col * 2, 0, 0)); }
+    // results of the tensors' own type: one rounding
+    VA_DEVINL void put(int row, int col, float x) const { __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(x), c.r, row * c.row + col * 2, 0, 0); }
 };
-template <typename T> VA_DEVINL f32x4_t load4(const T* p) { return widen4(*(const typename elem<T>::raw4*)p); }
+template <typename T> VA_DEVINL ChunkOf<T> chunk_of(const T* first, int64_t ld, int rows) {
+    return ChunkOf<T>{chunk_base(first, ld * (int64_t)sizeof(T), rows)};
+}
 
 // where a token's row of one head lies: rows of `ld` elements, heads side by side
 struct Rows {
     int64_t ld;
     VA_DEVINL int64_t at(int64_t b, int64_t L, int64_t t, int64_t h, int64_t hd) const { return (b * L + t) * ld + h * hd; }
 };
+// Chunk of a workgroup in the kernels that take all chunks at once: the heads of a token are neighbours in memory, so
+// neighbouring workgroups take them (one head's rows alone keep to few memory channels).
+VA_DEVINL void chunk_place(int64_t id, int H, int NC, int64_t& b, int& h, int& c) {
+    h = (int)(id % H);
+    c = (int)(id / H % NC);
+    b = id / H / NC;
+}
 
-// Decays of a chunk.  a[] in LDS (1 behind the sequence's end).  Lane i of one wave walks the tokens back from i:
+// how many bf16 numbers stand for an input element, for an intermediate, and for an operand of an output
+template <typename T> struct parts;
+template <> struct parts<float> { static constexpr int IN = 3, MID = 3, OUT = 3; };
+template <> struct parts<bf16_t> { static constexpr int IN = 1, MID = 3, OUT = 2; };
+
+// eight f32 values (two accumulator tiles of a lane) -> N operands of eight bf16 numbers each
+template <int N>
+VA_DEVINL void split(f32x4_t a, f32x4_t b, bf16x8_t (&out)[N]) {
+    float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        u32x4_t w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+            x[2 * e] -= __uint_as_float(w[e] << 16);
+            x[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+        }
+        out[n] = __builtin_bit_cast(bf16x8_t, w);
+    }
+}
+// acc[x] += a[x] * b from their parts, every pair whose product is above 2^-24 of the whole; independent accumulators follow
+// each other
+template <int X, int NA, int NB>
+VA_DEVINL void mfma_parts_of(const bf16x8_t (&a)[X][NA], const bf16x8_t (&b)[NB], f32x4_t* acc) {
+    constexpr int KEEP = NA > NB ? NA : NB;
+#pragma unroll
+    for (int i = NA - 1; i >= 0; --i)
+#pragma unroll
+        for (int j = NB - 1; j >= 0; --j)
+            if (i + j < KEEP) {
+#pragma unroll
+                for (int x = 0; x < X; ++x) acc[x] = mfma16(a[x][i], b[j], acc[x]);
+            }
+}
+// operand blocks: (row tile it, columns 32u..) of a lower triangle, and of an upper one
+__host__ __device__ constexpr int low_block(int it, int u) { return it < 2 ? it : 2 * it - 2 + u; }
+__host__ __device__ constexpr int up_block(int jt, int u) { return jt < 2 ? 2 * jt + u : 2 + jt; }
+template <int N>
+VA_DEVINL void load_block(const char* base, int block, int lane, bf16x8_t (&out)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) out[n] = *(const bf16x8_t*)(base + (block * N + n) * BFRAG * 2 + lane * 16);
+}
+// acc[first..] += (row tiles first..first + X - 1, column block u) of an operand in LDS times b
+template <int X, bool UP, int NA, int NB>
+VA_DEVINL void blocks_times(const char* base, int first, int u, const bf16x8_t (&b)[NB], f32x4_t* acc, int lane) {
+    bf16x8_t a[X][NA];
+#pragma unroll
+    for (int x = 0; x < X; ++x) load_block(base, UP ? up_block(first + x, u) : low_block(first + x, u), lane, a[x]);
+    mfma_parts_of<X>(a, b, acc + first);
+}
+template <int N>
+VA_DEVINL void store_block(bf16_t* base, int block, int lane, const bf16x8_t (&v)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) *(bf16x8_t*)(base + (block * N + n) * BFRAG + lane * 8) = v[n];
+}
+
+// Decays of a chunk, `mine` = lane's own a (1 behind the sequence's end): lane i of one wave walks the tokens back from i,
 // gt[j][i] = a_{j+1} ... a_i for j <= i, 0 above.
-VA_DEVINL void chunk_decays(const float* a, float (*gt)[SQ], int lane) {
+VA_DEVINL void chunk_decays(float mine, float (*gt)[SQ], int lane) {
     float p = 0.f;
+#pragma unroll
     for (int j = DC - 1; j >= 0; --j) {
-        p = j == lane ? 1.0f : j < lane ? p * a[j + 1] : 0.f;      // j < lane: j + 1 is inside the chunk
+        if (j + 1 < DC) p *= __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), j + 1));
+        p = j == lane ? 1.0f : j < lane ? p : 0.f;
         gt[j][lane] = p;
     }
 }
 // lane i: a_0 ... a_i
-VA_DEVINL float chunk_prefix(const float* a, int lane) {
-    float p = 1.f, mine = 1.f;
-    for (int j = 0; j < DC; ++j) {
-        p *= a[j];
-        mine = j == lane ? p : mine;
+VA_DEVINL float chunk_prefix(float mine, int lane) {
+    float p = mine;
+#pragma unroll
+    for (int off = 1; off < DC; off <<= 1) {
+        const float q = __shfl_up(p, off);
+        p = lane >= off ? p * q : p;
     }
-    return mine;
+    return p;
 }
 
-template <int HD, typename T, int THREADS>
-VA_DEVINL void rows_to_lds(const T* __restrict__ src, int64_t first, int64_t ld, int rows_left, float (*dst)[HD + 4], int tid) {
-    constexpr int N = DC * HD / 4 / THREADS;
+template <int HD, typename T>
+VA_DEVINL void rows_to_lds(const ChunkOf<T>& src, float (*dst)[HD + 4], int tid) {
+    constexpr int N = DC * HD / 4 / 256;
 #pragma unroll
     for (int p = 0; p < N; ++p) {
-        const int idx = p * THREADS + tid, row = idx / (HD / 4), c = (idx % (HD / 4)) * 4;
-        f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-        if (row < rows_left) v = load4(src + first + (int64_t)row * ld + c);
-        *(f32x4_t*)&dst[row][c] = v;
+        const int idx = p * 256 + tid, row = idx / (HD / 4), c = (idx % (HD / 4)) * 4;
+        *(f32x4_t*)&dst[row][c] = widen4(src.raw(row, c));
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// One workgroup of four waves per chunk.  Tiles are formed transposed, D[j][i] = k_j.x_i, so that a lane holds row i and
-// four consecutive j: the operand order in which T and P are kept.  GRAD: T, T^T and P^T for the gradient's scans,
-// otherwise T and P.
+// One workgroup of four waves per chunk.  K K^T tiles are formed transposed, D[j][i] = k_j.k_i, so that a lane holds row i and
+// four consecutive j; the wave with row tile w of K K^T (w + 1 tiles) takes row tile 3 - w of Q K^T, five tiles to each.  GRAD:
+// T, T^T and P^T for the gradient's scans (then by column tiles, P^T's rows: 4 - w tiles), otherwise T and P.
 template <int HD, typename T, bool GRAD>
 __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q, const T* __restrict__ K, Rows rq, Rows rk,
                                                          const float* __restrict__ ALPHA, const float* __restrict__ BETA,
-                                                         float* __restrict__ TF, float* __restrict__ TT, float* __restrict__ PF,
+                                                         bf16_t* __restrict__ TF, bf16_t* __restrict__ TT, bf16_t* __restrict__ PF,
                                                          float* __restrict__ GAM, int L, int H, int NC) {
-    extern __shared__ __align__(16) char lds[];
+    constexpr int NM = parts<T>::MID, NP = GRAD ? parts<T>::MID : parts<T>::OUT;
+    constexpr int KBYTES = DC * (HD + 4) * 4, ABYTES = DC * SQ * 4 + DC * 20 * 4;
+    __shared__ __align__(16) char lds[(KBYTES > ABYTES ? KBYTES : ABYTES)];
+    __shared__ float gt[DC][SQ];
+    __shared__ float sb[DC];
     float(*ks)[HD + 4] = (float(*)[HD + 4])lds;
-    float(*qs)[HD + 4] = ks + DC;
-    float(*gt)[SQ] = (float(*)[SQ])(qs + DC);
-    float(*am)[SQ] = gt + DC;                     // A, then T
+    float(*am)[SQ] = (float(*)[SQ])lds;           // A, then T: over K, which is not needed by then
     float(*dg)[20] = (float(*)[20])(am + DC);     // inverses of the four diagonal blocks of I + A
-    float* sa = (float*)(dg + DC);
-    float* sb = sa + DC;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g4 = (lane >> 4) * 4;
-    const int64_t ci = blockIdx.x;
-    const int64_t bh = ci / NC;
-    const int c = (int)(ci % NC), t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
-    const int64_t b = bh / H, h = bh % H;
-    rows_to_lds<HD, T, 256>(K, rk.at(b, L, t0, h, HD), rk.ld, left, ks, tid);
-    rows_to_lds<HD, T, 256>(Q, rq.at(b, L, t0, h, HD), rq.ld, left, qs, tid);
-    if (tid < DC) {
-        const int64_t at = (b * L + t0 + tid) * H + h;
-        sa[tid] = tid < left ? ALPHA[at] : 1.0f;
-        sb[tid] = tid < left ? BETA[at] : 0.0f;
-    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g4 = (lane >> 4) * 4;
+    int64_t b;
+    int h, c;
+    chunk_place(blockIdx.x, H, NC, b, h, c);
+    const int64_t ci = (b * H + h) * NC + c;
+    const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
+    const ChunkOf<T> qc = chunk_of(Q + rq.at(b, L, t0, h, HD), rq.ld, left);
+    rows_to_lds<HD, T>(chunk_of(K + rk.at(b, L, t0, h, HD), rk.ld, left), ks, tid);
+    const float mine = lane < left ? ALPHA[(b * L + t0 + lane) * H + h] : 1.0f;
+    if (tid < DC) sb[tid] = tid < left ? BETA[(b * L + t0 + tid) * H + h] : 0.0f;
+    if (wave == 0) chunk_decays(mine, gt, lane);
+    if (wave == 1) GAM[ci * 2 * DC + lane] = chunk_prefix(mine, lane);
     __syncthreads();
-    if (wave == 0) chunk_decays(sa, gt, lane);
-    if (wave == 1) GAM[ci * 2 * DC + lane] = chunk_prefix(sa, lane);
-    f32x4_t acc[5];                               // 20 tiles (K K^T and Q K^T), five to a wave
+    const int qt = GRAD ? wave : 3 - wave;        // this wave's rows of Q (GRAD: its rows of P^T)
+    f32x4_t kk[4], qk[4];                         // kk[jt]: rows `wave`; qk[jt]: rows qt (GRAD: qk[it], P^T's columns)
 #pragma unroll
-    for (int s = 0; s < 5; ++s) {
-        const int x = wave + 4 * s, tile = x % TRI;
-        const int it = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, jt = tile - tri(it, 0);
-        const bool qk = x >= TRI;
-        const float* rj = ks[16 * jt + m] + g4;
-        const float* ri = (qk ? qs : ks)[16 * it + m] + g4;
-        // P^T for the gradient: lane holds row j and four consecutive i
-        const float* ra = qk && GRAD ? ri : rj;
-        const float* rb = qk && GRAD ? rj : ri;
-        f32x4_t d = {0.f, 0.f, 0.f, 0.f}, e = d;
+    for (int x = 0; x < 4; ++x) kk[x] = qk[x] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    // one copy of the code per wave: which tiles it forms is then known to the compiler
+    auto tiles = [&](auto wv) {
+        constexpr int WV = decltype(wv)::value, QT = GRAD ? WV : 3 - WV;
 #pragma unroll
         for (int u = 0; u < HD / 16; ++u) {
-            const f32x4_t x4 = *(const f32x4_t*)(ra + 16 * u), y4 = *(const f32x4_t*)(rb + 16 * u);
-            d = mfma_f32(x4[0], y4[0], d);
-            e = mfma_f32(x4[1], y4[1], e);
-            d = mfma_f32(x4[2], y4[2], d);
-            e = mfma_f32(x4[3], y4[3], e);
-        }
-        acc[s] = d + e;
-    }
-    __syncthreads();                              // the decays are there
-    if (wave == 2) GAM[ci * 2 * DC + DC + lane] = gt[lane][DC - 1];
+            const int col = 16 * u + g4;
+            const f32x4_t mk = *(const f32x4_t*)&ks[16 * WV + m][col];
+            f32x4_t mq = mk;                      // GRAD: the rows of P^T are keys, the wave's own
+            if (!GRAD) mq = widen4(qc.raw(16 * QT + m, col));
 #pragma unroll
-    for (int s = 0; s < 5; ++s) {
-        const int x = wave + 4 * s, tile = x % TRI;
-        const int it = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, jt = tile - tri(it, 0);
-        f32x4_t v = acc[s];
-        if (x < TRI) {
-            const int i = 16 * it + m;
+            for (int x = 0; x < 4; ++x) {
+                f32x4_t kx = {0.f, 0.f, 0.f, 0.f}, qx = kx;
+                if (x <= WV || (!GRAD && x <= QT)) kx = *(const f32x4_t*)&ks[16 * x + m][col];
+                if (GRAD && x >= WV) qx = widen4(qc.raw(16 * x + m, col));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (x <= WV) kk[x] = mfma_f32(kx[r], mk[r], kk[x]);
+                    if (!GRAD && x <= QT) qk[x] = mfma_f32(kx[r], mq[r], qk[x]);
+                    if (GRAD && x >= WV) qk[x] = mfma_f32(qx[r], mq[r], qk[x]);
+                }
+            }
+        }
+    };
+    if (wave == 0) tiles(int_c<0>{});
+    else if (wave == 1) tiles(int_c<1>{});
+    else if (wave == 2) tiles(int_c<2>{});
+    else tiles(int_c<3>{});
+    __syncthreads();                              // K has been read
+    if (wave == 2) GAM[ci * 2 * DC + DC + lane] = gt[lane][DC - 1];
+    {
+        const int i = 16 * wave + m;
+        const float bi = sb[i];
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt) {
+            if (jt > wave) continue;
+            f32x4_t v;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int j = 16 * jt + g4 + r;
-                v[r] = i > j ? v[r] * sb[i] * gt[j][i] : 0.f;
+                v[r] = i > j ? kk[jt][r] * bi * gt[j][i] : 0.f;
             }
             *(f32x4_t*)&am[i][16 * jt + g4] = v;
-        } else {
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = GRAD ? 16 * it + g4 + r : 16 * it + m, j = GRAD ? 16 * jt + m : 16 * jt + g4 + r;
-                v[r] *= gt[j][i];                 // 0 above the diagonal
+                const int ii = GRAD ? 16 * x + g4 + r : 16 * qt + m, j = GRAD ? 16 * wave + m : 16 * x + g4 + r;
+                qk[x][r] = ii >= j ? qk[x][r] * gt[j][ii] : 0.f;
             }
-            *(f32x4_t*)(PF + (ci * TRI + tile) * FRAG + lane * 4) = v;
-        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (GRAD ? 2 * u + 1 >= wave : 2 * u <= qt) {
+                bf16x8_t f[NP];
+                split(qk[2 * u], qk[2 * u + 1], f);
+                store_block(PF + ci * BLK * NP * BFRAG, GRAD ? up_block(wave, u) : low_block(qt, u), lane, f);
+            }
     }
     __syncthreads();
     // inverse of a diagonal block by forward substitution, lane = column
@@ -190,168 +298,265 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q
     __syncthreads();
     // the blocks below, by block columns: X_ij = -D_i sum_{j <= k < i} A_ik X_kj; a block column per wave, in registers
     f32x4_t xb[4];
-    {
-        const int jt = wave;
+    auto column = [&](auto wv) {
+        constexpr int JT = decltype(wv)::value;
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
-            if (it < jt) continue;
-            if (it == jt) {
+            xb[it] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            if (it == JT) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) xb[it][r] = dg[16 * it + g4 + r][m];
-                continue;
             }
-            f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+            if (it > JT) {
+                f32x4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int kt = 0; kt < it; ++kt) {
-                if (kt < jt) continue;
-                const f32x4_t a4 = *(const f32x4_t*)&am[16 * it + m][16 * kt + g4];
+                for (int kt = JT; kt < it; ++kt) {
+                    const f32x4_t a4 = *(const f32x4_t*)&am[16 * it + m][16 * kt + g4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s = mfma_f32(a4[r], xb[kt][r], s);
+                    for (int r = 0; r < 4; ++r) s = mfma_f32(a4[r], xb[kt][r], s);
+                }
+                const f32x4_t d4 = *(const f32x4_t*)&dg[16 * it + m][g4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) xb[it] = mfma_f32(-d4[r], s[r], xb[it]);
             }
-            const f32x4_t d4 = *(const f32x4_t*)&dg[16 * it + m][g4];
-            f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o = mfma_f32(-d4[r], s[r], o);
-            xb[it] = o;
         }
+    };
+    if (wave == 0) column(int_c<0>{});
+    else if (wave == 1) column(int_c<1>{});
+    else if (wave == 2) column(int_c<2>{});
+    else column(int_c<3>{});
+    __syncthreads();
+#pragma unroll
+    for (int it = 0; it < 4; ++it)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) am[16 * it + g4 + r][16 * wave + m] = xb[it][r];     // zeros above the diagonal too
+    if (GRAD) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (2 * u + 1 >= wave) {
+                bf16x8_t f[NM];
+                split(xb[2 * u], xb[2 * u + 1], f);
+                store_block(TT + ci * BLK * NM * BFRAG, up_block(wave, u), lane, f);
+            }
     }
     __syncthreads();
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {
-        if (it < wave) continue;
-        if (GRAD) *(f32x4_t*)(TT + (ci * TRI + tri(it, wave)) * FRAG + lane * 4) = xb[it];
+    for (int u = 0; u < 2; ++u)
+        if (2 * u <= wave) {
+            const float* row = am[16 * wave + m] + 32 * u + g4;
+            bf16x8_t f[NM];
+            split(*(const f32x4_t*)row, *(const f32x4_t*)(row + 16), f);
+            store_block(TF + ci * BLK * NM * BFRAG, low_block(wave, u), lane, f);
+        }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// A chunk's rows in LDS as bf16 parts, plane n of a matrix at [n][row], rows of HD * 2 bytes in 16-byte pieces.  Columns
+// 32u + 16h + 4g + r of a row are element 4h + r of piece 4u + g, so one 16-byte read is a left operand's eight elements; the
+// pieces of row t stand at (piece ^ turn(t)), which spreads the sixteen rows of such a read, and the four rows times four
+// pieces of a transposed one, over all banks.
+template <int HD> VA_DEVINL int turn(int row) {
+    return HD == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+}
+template <int HD> VA_DEVINL int piece_at(int row, int piece) { return row * HD * 2 + ((piece ^ turn<HD>(row)) << 4); }
+// columns 4c .. 4c+3 of a row
+template <int HD> VA_DEVINL int quad_at(int row, int c) { return piece_at<HD>(row, (c >> 3) * 4 + (c & 3)) + ((c >> 2) & 1) * 8; }
+
+VA_DEVINL void put_rows(char* at, int plane, f32x4_t v) {        // f32: three parts
+    float x[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) am[16 * it + g4 + r][16 * wave + m] = xb[it][r];
+    for (int n = 0; n < 3; ++n) {
+        const u32x2_t w = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+        *(u32x2_t*)(at + n * plane) = w;
+        x[0] -= __uint_as_float(w[0] << 16);
+        x[1] -= __uint_as_float(w[0] & 0xffff0000u);
+        x[2] -= __uint_as_float(w[1] << 16);
+        x[3] -= __uint_as_float(w[1] & 0xffff0000u);
     }
-    __syncthreads();
-    for (int x = wave; x < TRI; x += 4) {
-        const int it = x < 1 ? 0 : x < 3 ? 1 : x < 6 ? 2 : 3, jt = x - tri(it, 0);
-        *(f32x4_t*)(TF + (ci * TRI + x) * FRAG + lane * 4) = *(const f32x4_t*)&am[16 * it + m][16 * jt + g4];
+}
+VA_DEVINL void put_rows(char* at, int, u32x2_t v) { *(u32x2_t*)at = v; }
+
+// left operand of rows 16 it.., columns 32u + 4g + {0..3, 16..19}
+template <int HD, int N>
+VA_DEVINL void row_frag(const char* x, int it, int u, int m, int g, bf16x8_t (&out)[N]) {
+    const char* at = x + piece_at<HD>(16 * it + m, 4 * u + g);
+#pragma unroll
+    for (int n = 0; n < N; ++n) out[n] = *(const bf16x8_t*)(at + n * DC * HD * 2);
+}
+// left operand of the transposed rows: columns 16 ct.. of x, tokens 32u + 4g + {0..3, 16..19}
+template <int HD, int N>
+VA_DEVINL void col_frag(const char* x, int ct, int u, int lane, bf16x8_t (&out)[N]) {
+    const int q = (lane & 15) >> 2, p = lane & 3, g = lane >> 4;
+    const char* lo = x + quad_at<HD>(32 * u + 4 * g + q, 4 * ct + p);
+    const char* hi = x + quad_at<HD>(32 * u + 16 + 4 * g + q, 4 * ct + p);
+#pragma unroll
+    for (int n = 0; n < N; ++n) out[n] = join_tr(lds_read_tr16(lo + n * DC * HD * 2), lds_read_tr16(hi + n * DC * HD * 2));
+}
+
+// a workgroup's LDS writes are there; loads under way stay under way
+VA_DEVINL void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// `bytes` (whole kilobytes) from memory to LDS without registers, a kilobyte per wave and step; the buffer form's LDS
+// destination is one the compiler knows, so other LDS reads do not wait for it
+template <int BYTES, int W>
+VA_DEVINL void to_lds(const void* src, char* dst, int wave, int lane) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)src, (short)0, BYTES, 0x00020000);
+#pragma unroll
+    for (int x = 0; x < (BYTES / 1024 + W - 1) / W; ++x) {
+        const int kb = x * W + wave;
+        if (BYTES / 1024 % W == 0 || kb < BYTES / 1024)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)(dst + kb * 1024), 16, kb * 1024 + lane * 16, 0, 0, 0);
     }
 }
 
-// acc[it] += X (64 rows, HD columns, in LDS) * B, B = accumulator tiles
-template <int HD>
-VA_DEVINL void rows_times_tiles(const float (*x)[HD + 4], const f32x4_t* bt, f32x4_t* acc, int m, int g4) {
+// What the two scans share: the next chunk's rows of K (and Q) on their way from memory to LDS.  LDS of a workgroup: K, Q, the
+// chunk's two 64x64 operands (NA and NB parts), b, g, g_C.
+template <int HD, typename T, int W, bool TWO, int NA, int NB>
+struct ChunkRows {
+    typedef typename ChunkOf<T>::raw4 raw4;
+    static constexpr int N = DC * HD / 4 / (64 * W), IN = parts<T>::IN, MATRIX = IN * DC * HD * 2;
+    static constexpr int A_BYTES = BLK * NA * BFRAG * 2, B_BYTES = BLK * NB * BFRAG * 2;
+    static constexpr int A_AT = (TWO ? 2 : 1) * MATRIX, B_AT = A_AT + A_BYTES, F_AT = B_AT + B_BYTES, LDS = F_AT + 3 * DC * 4;
+    const T *k, *q;                               // row 0 of this head
+    int64_t ldk, ldq;
+    const float *beta, *gam;
+    int L, H, tid;
+    raw4 kn[N], qn[TWO ? N : 1];
+    float bn, gn, en;
+    VA_DEVINL void request(int c, int NC) {       // a chunk outside the sequence: nothing is read
+        const bool inside = c >= 0 && c < NC;
+        c = inside ? c : 0;
+        const int left = inside ? (L - c * DC < DC ? L - c * DC : DC) : 0;
+        const ChunkOf<T> kc = chunk_of(k + (int64_t)c * DC * ldk, ldk, left), qc = chunk_of(q + (int64_t)c * DC * ldq, ldq, left);
 #pragma unroll
-    for (int u = 0; u < HD / 16; ++u) {
-        f32x4_t a[4];
-#pragma unroll
-        for (int it = 0; it < 4; ++it) a[it] = *(const f32x4_t*)&x[16 * it + m][16 * u + g4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int it = 0; it < 4; ++it) acc[it] = mfma_f32(a[it][r], bt[u][r], acc[it]);
+        for (int p = 0; p < N; ++p) {
+            const int idx = p * 64 * W + tid, row = idx / (HD / 4), col = (idx % (HD / 4)) * 4;
+            kn[p] = kc.raw(row, col);
+            if (TWO) qn[p] = qc.raw(row, col);
+        }
+        if (tid < DC) {
+            bn = tid < left ? beta[((int64_t)c * DC + tid) * H] : 0.f;
+            gn = gam[(int64_t)c * 2 * DC + tid];  // (chunk 0's instead)
+            en = gam[(int64_t)c * 2 * DC + DC + tid];
+        }
     }
+    VA_DEVINL void place(char* lds) {
+#pragma unroll
+        for (int p = 0; p < N; ++p) {
+            const int idx = p * 64 * W + tid, at = quad_at<HD>(idx / (HD / 4), idx % (HD / 4));
+            put_rows(lds + at, DC * HD * 2, kn[p]);
+            if (TWO) put_rows(lds + MATRIX + at, DC * HD * 2, qn[p]);
+        }
+        float* f = (float*)(lds + F_AT);
+        if (tid < DC) f[tid] = bn, f[DC + tid] = gn, f[2 * DC + tid] = en;
+    }
+};
+
+// acc[ct] += X^T B for all HD/16 column tiles of X, B in parts
+template <int HD, int NX, int NB>
+VA_DEVINL void columns_times(const char* x, const bf16x8_t (&bt)[2][NB], f32x4_t* acc, int lane) {
+#pragma unroll
+    for (int ct = 0; ct < HD / 16; ct += 2)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            bf16x8_t a[2][NX];
+            col_frag<HD>(x, ct, u, lane, a[0]);
+            col_frag<HD>(x, ct + 1, u, lane, a[1]);
+            mfma_parts_of<2>(a, bt[u], acc + ct);
+        }
 }
-// acc[u] += X^T (HD rows, 64 columns) * B
-template <int HD>
-VA_DEVINL void columns_times_tiles(const float (*x)[HD + 4], const f32x4_t* bt, f32x4_t* acc, int m, int g4) {
+// acc[it] += rows of X times B (tiles it, column block u)
+template <int HD, int NX, int NB>
+VA_DEVINL void rows_times(const char* x, int u, const bf16x8_t (&bt)[NB], f32x4_t* acc, int m, int g) {
+    bf16x8_t a[4][NX];
 #pragma unroll
-    for (int jt = 0; jt < 4; ++jt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int u = 0; u < HD / 16; ++u) acc[u] = mfma_f32(x[16 * jt + g4 + r][16 * u + m], bt[jt][r], acc[u]);
+    for (int it = 0; it < 4; ++it) row_frag<HD>(x, it, u, m, g, a[it]);
+    mfma_parts_of<4>(a, bt, acc);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // The sequential part.  A wave owns 16 columns (values of the head) of the state for the whole sequence: M in HD/16
-// accumulator tiles; W waves share a chunk's K and Q through LDS.  The next chunk's rows are requested before the
-// current one computes.  OUT: writes o.  SAVE: writes U and every chunk's starting state (rows of S) for the gradient.
+// accumulator tiles; W waves share a chunk's K, Q, T and P through LDS.  K and Q of the next chunk are requested half-way
+// through the current one, T and P of a chunk arrive while its products with M are formed.
+// OUT: writes o.  SAVE: writes U and every chunk's starting state (rows of S) for the gradient.
 template <int HD, typename T, int W, bool OUT, bool SAVE>
 __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                                                             Rows rq, Rows rk, Rows rv, const float* __restrict__ BETA,
-                                                            const float* __restrict__ TF, const float* __restrict__ PF,
+                                                            const bf16_t* __restrict__ TF, const bf16_t* __restrict__ PF,
                                                             const float* __restrict__ GAM, const float* __restrict__ STATE_IN,
                                                             T* __restrict__ O, float* __restrict__ STATE_OUT,
                                                             float* __restrict__ US, float* __restrict__ MS, int L, int H, int NC) {
+    constexpr int NI = parts<T>::IN, NM = parts<T>::MID, NO = parts<T>::OUT;
+    typedef ChunkRows<HD, T, W, OUT, NM, OUT ? NO : 0> CR;
     extern __shared__ __align__(16) char lds[];
-    float(*ks)[HD + 4] = (float(*)[HD + 4])lds;
-    float(*qs)[HD + 4] = ks + DC;
-    float* sb = (float*)(ks + (OUT ? 2 : 1) * DC);
-    float* sg = sb + DC;
-    float* se = sg + DC;
-    constexpr int GROUPS = HD / 16 / W, N = DC * HD / 4 / (64 * W);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g4 = (lane >> 4) * 4;
+    const char *ks = lds, *qs = lds + CR::MATRIX;
+    char *tl = lds + CR::A_AT, *pl = lds + CR::B_AT;
+    const float *sb = (const float*)(lds + CR::F_AT), *sg = sb + DC, *se = sg + DC;
+    constexpr int GROUPS = HD / 16 / W;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4, g4 = g * 4;
     const int wid = xcd_remap(blockIdx.x, gridDim.x);
     const int64_t bh = wid / GROUPS, b = bh / H, h = bh % H;
     const int v = ((wid % GROUPS) * W + wave) * 16 + m;
-    const int64_t qrow = rq.at(b, L, 0, h, HD), krow = rk.at(b, L, 0, h, HD), vrow = rv.at(b, L, 0, h, HD);
-    typedef typename elem<T>::raw4 raw4;
-    raw4 kn[N], qn[N];
-    float bn = 0.f, gn = 0.f, en = 0.f;
-    auto request = [&](int c) {
-        const int left = L - c * DC;
-#pragma unroll
-        for (int p = 0; p < N; ++p) {
-            const int idx = p * 64 * W + tid, row = idx / (HD / 4), col = (idx % (HD / 4)) * 4;
-            const int64_t t = (int64_t)c * DC + row;
-            kn[p] = raw4{};
-            if (row < left) kn[p] = *(const raw4*)(K + krow + t * rk.ld + col);
-            if (OUT) {
-                qn[p] = raw4{};
-                if (row < left) qn[p] = *(const raw4*)(Q + qrow + t * rq.ld + col);
-            }
-        }
-        if (tid < DC) {
-            bn = tid < left ? BETA[(b * L + (int64_t)c * DC + tid) * H + h] : 0.f;
-            gn = GAM[(bh * NC + c) * 2 * DC + tid];
-            en = GAM[(bh * NC + c) * 2 * DC + DC + tid];
-        }
-    };
+    const T* vb = V + rv.at(b, L, 0, h, HD);
+    CR cr;
+    cr.k = K + rk.at(b, L, 0, h, HD), cr.q = Q + rq.at(b, L, 0, h, HD), cr.ldk = rk.ld, cr.ldq = rq.ld;
+    cr.beta = BETA + b * L * H + h, cr.gam = GAM + bh * NC * 2 * DC, cr.L = L, cr.H = H, cr.tid = tid;
     f32x4_t M[HD / 16];
 #pragma unroll
     for (int u = 0; u < HD / 16; ++u) {
         M[u] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
         if (STATE_IN != nullptr) M[u] = *(const f32x4_t*)(STATE_IN + (bh * HD + v) * HD + 16 * u + g4);
     }
-    request(0);
+    cr.request(0, NC);
     for (int c = 0; c < NC; ++c) {
-        const int t0 = c * DC, left = L - t0;
+        const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
         const int64_t ci = bh * NC + c;
         __syncthreads();                          // everybody is done with the chunk before
-#pragma unroll
-        for (int p = 0; p < N; ++p) {
-            const int idx = p * 64 * W + tid, row = idx / (HD / 4), col = (idx % (HD / 4)) * 4;
-            *(f32x4_t*)&ks[row][col] = widen4(kn[p]);
-            if (OUT) *(f32x4_t*)&qs[row][col] = widen4(qn[p]);
-        }
-        if (tid < DC) sb[tid] = bn, sg[tid] = gn, se[tid] = en;
-        __syncthreads();
-        // this chunk's v column (C order) and T, requested ahead of their use
-        f32x4_t vv[4], tf[TRI];
+        cr.place(lds);
+        to_lds<CR::A_BYTES, W>(TF + ci * BLK * NM * BFRAG, tl, wave, lane);
+        if (OUT) to_lds<CR::B_BYTES, W>(PF + ci * BLK * NO * BFRAG, pl, wave, lane);
+        f32x4_t vv[4];                            // this chunk's v column, rows in accumulator order
+        const ChunkOf<T> vc = chunk_of(vb + (int64_t)t0 * rv.ld, rv.ld, left);
 #pragma unroll
         for (int it = 0; it < 4; ++it)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * it + g4 + r;
-                vv[it][r] = i < left ? elem<T>::get(V + vrow + (int64_t)(t0 + i) * rv.ld + v) : 0.f;
-            }
-#pragma unroll
-        for (int x = 0; x < TRI; ++x) tf[x] = *(const f32x4_t*)(TF + (ci * TRI + x) * FRAG + lane * 4);
-        if (c + 1 < NC) request(c + 1);
+            for (int r = 0; r < 4; ++r) vv[it][r] = vc.get(16 * it + g4 + r, v);
+        lds_barrier();
         if (SAVE) {
 #pragma unroll
             for (int u = 0; u < HD / 16; ++u) *(f32x4_t*)(MS + (ci * HD + v) * HD + 16 * u + g4) = M[u];
         }
-        f32x4_t rhs[4], U[4];
+        f32x4_t rhs[4], o[4], U[4];
 #pragma unroll
-        for (int it = 0; it < 4; ++it) rhs[it] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-        rows_times_tiles<HD>(ks, M, rhs, m, g4);
+        for (int it = 0; it < 4; ++it) rhs[it] = o[it] = U[it] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < HD / 32; ++u) {
+            bf16x8_t mf[NM], mo[NO];
+            split(M[2 * u], M[2 * u + 1], mf);
+            rows_times<HD, NI>(ks, u, mf, rhs, m, g);
+            if (OUT) {
+#pragma unroll
+                for (int n = 0; n < NO; ++n) mo[n] = mf[n];
+                rows_times<HD, NI>(qs, u, mo, o, m, g);
+            }
+        }
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
             const f32x4_t b4 = *(const f32x4_t*)(sb + 16 * it + g4), gg = *(const f32x4_t*)(sg + 16 * it + g4);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) rhs[it][r] = b4[r] * (vv[it][r] - gg[r] * rhs[it][r]);
-            U[it] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            for (int r = 0; r < 4; ++r) {
+                rhs[it][r] = b4[r] * (vv[it][r] - gg[r] * rhs[it][r]);
+                o[it][r] *= gg[r];
+            }
         }
+        bf16x8_t f[2][NM];
 #pragma unroll
-        for (int jt = 0; jt < 4; ++jt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int it = jt; it < 4; ++it) U[it] = mfma_f32(tf[tri(it, jt)][r], rhs[jt][r], U[it]);
+        for (int u = 0; u < 2; ++u) split(rhs[2 * u], rhs[2 * u + 1], f[u]);
+        wait_vm0();
+        __syncthreads();                          // T and P are there
+        cr.request(c + 1, NC);
+        blocks_times<4, false, NM>(tl, 0, 0, f[0], U, lane);
+        blocks_times<2, false, NM>(tl, 2, 1, f[1], U, lane);
         if (SAVE) {
 #pragma unroll
             for (int it = 0; it < 4; ++it)
@@ -359,34 +564,25 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
                 for (int r = 0; r < 4; ++r) US[(ci * DC + 16 * it + g4 + r) * HD + v] = U[it][r];
         }
         if (OUT) {
-            f32x4_t pf[TRI], o[4];
+            bf16x8_t uf[2][NO];
 #pragma unroll
-            for (int x = 0; x < TRI; ++x) pf[x] = *(const f32x4_t*)(PF + (ci * TRI + x) * FRAG + lane * 4);
-#pragma unroll
-            for (int it = 0; it < 4; ++it) o[it] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-            rows_times_tiles<HD>(qs, M, o, m, g4);
-#pragma unroll
-            for (int it = 0; it < 4; ++it) o[it] *= *(const f32x4_t*)(sg + 16 * it + g4);
-#pragma unroll
-            for (int jt = 0; jt < 4; ++jt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int it = jt; it < 4; ++it) o[it] = mfma_f32(pf[tri(it, jt)][r], U[jt][r], o[it]);
+            for (int u = 0; u < 2; ++u) split(U[2 * u], U[2 * u + 1], uf[u]);
+            blocks_times<4, false, NO>(pl, 0, 0, uf[0], o, lane);
+            blocks_times<2, false, NO>(pl, 2, 1, uf[1], o, lane);
+            const ChunkOf<T> oc = chunk_of((const T*)O + ((b * L + t0) * H + h) * HD, (int64_t)H * HD, left);
 #pragma unroll
             for (int it = 0; it < 4; ++it)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * it + g4 + r;
-                    if (i < left) elem<T>::put(O + ((b * L + t0 + i) * H + h) * HD + v, o[it][r]);
-                }
+                for (int r = 0; r < 4; ++r) oc.put(16 * it + g4 + r, v, o[it][r]);
         }
         const float gc = sg[DC - 1];
 #pragma unroll
         for (int u = 0; u < HD / 16; ++u) M[u] *= gc;
 #pragma unroll
         for (int it = 0; it < 4; ++it) U[it] *= *(const f32x4_t*)(se + 16 * it + g4);
-        columns_times_tiles<HD>(ks, U, M, m, g4);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) split(U[2 * u], U[2 * u + 1], f[u]);
+        columns_times<HD, NI>(ks, f, M, lane);
     }
     if (STATE_OUT != nullptr) {
 #pragma unroll
@@ -399,100 +595,74 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
 template <int HD, typename T, int W>
 __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict__ Q, const T* __restrict__ K, Rows rq, Rows rk,
                                                              const T* __restrict__ DO, const float* __restrict__ BETA,
-                                                             const float* __restrict__ TT, const float* __restrict__ PT,
+                                                             const bf16_t* __restrict__ TT, const bf16_t* __restrict__ PT,
                                                              const float* __restrict__ GAM, const float* __restrict__ DSTATE,
                                                              T* __restrict__ DV, float* __restrict__ DSTATE_IN,
                                                              float* __restrict__ RS, float* __restrict__ GS, int L, int H, int NC) {
+    constexpr int NI = parts<T>::IN, NM = parts<T>::MID;
+    typedef ChunkRows<HD, T, W, true, NM, NM> CR;
     extern __shared__ __align__(16) char lds[];
-    float(*ks)[HD + 4] = (float(*)[HD + 4])lds;
-    float(*qs)[HD + 4] = ks + DC;
-    float* sb = (float*)(qs + DC);
-    float* sg = sb + DC;
-    float* se = sg + DC;
-    constexpr int GROUPS = HD / 16 / W, N = DC * HD / 4 / (64 * W);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g4 = (lane >> 4) * 4;
+    const char *ks = lds, *qs = lds + CR::MATRIX;
+    char *pl = lds + CR::A_AT, *tl = lds + CR::B_AT;
+    const float *sb = (const float*)(lds + CR::F_AT), *sg = sb + DC, *se = sg + DC;
+    constexpr int GROUPS = HD / 16 / W;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4, g4 = g * 4;
     const int wid = xcd_remap(blockIdx.x, gridDim.x);
     const int64_t bh = wid / GROUPS, b = bh / H, h = bh % H;
     const int v = ((wid % GROUPS) * W + wave) * 16 + m;
-    const int64_t qrow = rq.at(b, L, 0, h, HD), krow = rk.at(b, L, 0, h, HD);
-    typedef typename elem<T>::raw4 raw4;
-    raw4 kn[N], qn[N];
-    float bn = 0.f, gn = 0.f, en = 0.f;
-    auto request = [&](int c) {
-        const int left = L - c * DC;
-#pragma unroll
-        for (int p = 0; p < N; ++p) {
-            const int idx = p * 64 * W + tid, row = idx / (HD / 4), col = (idx % (HD / 4)) * 4;
-            const int64_t t = (int64_t)c * DC + row;
-            kn[p] = raw4{};
-            qn[p] = raw4{};
-            if (row < left) {
-                kn[p] = *(const raw4*)(K + krow + t * rk.ld + col);
-                qn[p] = *(const raw4*)(Q + qrow + t * rq.ld + col);
-            }
-        }
-        if (tid < DC) {
-            bn = tid < left ? BETA[(b * L + (int64_t)c * DC + tid) * H + h] : 0.f;
-            gn = GAM[(bh * NC + c) * 2 * DC + tid];
-            en = GAM[(bh * NC + c) * 2 * DC + DC + tid];
-        }
-    };
+    CR cr;
+    cr.k = K + rk.at(b, L, 0, h, HD), cr.q = Q + rq.at(b, L, 0, h, HD), cr.ldk = rk.ld, cr.ldq = rq.ld;
+    cr.beta = BETA + b * L * H + h, cr.gam = GAM + bh * NC * 2 * DC, cr.L = L, cr.H = H, cr.tid = tid;
     f32x4_t G[HD / 16];
 #pragma unroll
     for (int u = 0; u < HD / 16; ++u) {
         G[u] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
         if (DSTATE != nullptr) G[u] = *(const f32x4_t*)(DSTATE + (bh * HD + v) * HD + 16 * u + g4);
     }
-    request(NC - 1);
+    cr.request(NC - 1, NC);
     for (int c = NC - 1; c >= 0; --c) {
-        const int t0 = c * DC, left = L - t0;
+        const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
         const int64_t ci = bh * NC + c;
-        __syncthreads();
-#pragma unroll
-        for (int p = 0; p < N; ++p) {
-            const int idx = p * 64 * W + tid, row = idx / (HD / 4), col = (idx % (HD / 4)) * 4;
-            *(f32x4_t*)&ks[row][col] = widen4(kn[p]);
-            *(f32x4_t*)&qs[row][col] = widen4(qn[p]);
-        }
-        if (tid < DC) sb[tid] = bn, sg[tid] = gn, se[tid] = en;
-        __syncthreads();
-        f32x4_t dov[4], pt[TRI], tt[TRI];
+        __syncthreads();                          // everybody is done with the chunk before
+        cr.place(lds);
+        to_lds<CR::A_BYTES, W>(PT + ci * BLK * NM * BFRAG, pl, wave, lane);
+        to_lds<CR::B_BYTES, W>(TT + ci * BLK * NM * BFRAG, tl, wave, lane);
+        f32x4_t dov[4];
+        const ChunkOf<T> oc = chunk_of(DO + ((b * L + t0) * H + h) * HD, (int64_t)H * HD, left);
 #pragma unroll
         for (int it = 0; it < 4; ++it)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * it + g4 + r;
-                dov[it][r] = i < left ? elem<T>::get(DO + ((b * L + t0 + i) * H + h) * HD + v) : 0.f;
-            }
-#pragma unroll
-        for (int x = 0; x < TRI; ++x) {
-            pt[x] = *(const f32x4_t*)(PT + (ci * TRI + x) * FRAG + lane * 4);
-            tt[x] = *(const f32x4_t*)(TT + (ci * TRI + x) * FRAG + lane * 4);
-        }
-        if (c > 0) request(c - 1);
+            for (int r = 0; r < 4; ++r) dov[it][r] = oc.get(16 * it + g4 + r, v);
+        lds_barrier();
 #pragma unroll
         for (int u = 0; u < HD / 16; ++u) *(f32x4_t*)(GS + (ci * HD + v) * HD + 16 * u + g4) = G[u];
         f32x4_t du[4], R[4];
 #pragma unroll
         for (int it = 0; it < 4; ++it) du[it] = R[it] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-        rows_times_tiles<HD>(ks, G, du, m, g4);
+#pragma unroll
+        for (int u = 0; u < HD / 32; ++u) {
+            bf16x8_t gf[NM];
+            split(G[2 * u], G[2 * u + 1], gf);
+            rows_times<HD, NI>(ks, u, gf, du, m, g);
+        }
 #pragma unroll
         for (int it = 0; it < 4; ++it) du[it] *= *(const f32x4_t*)(se + 16 * it + g4);
+        bf16x8_t of[2][NI], f[2][NM];
 #pragma unroll
-        for (int it = 0; it < 4; ++it)
+        for (int u = 0; u < 2; ++u) split(dov[2 * u], dov[2 * u + 1], of[u]);
+        wait_vm0();
+        __syncthreads();                          // P^T and T^T are there
+        cr.request(c - 1, NC);
+        blocks_times<2, true, NM>(pl, 0, 0, of[0], du, lane);
+        blocks_times<4, true, NM>(pl, 0, 1, of[1], du, lane);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int jt = 0; jt <= it; ++jt) du[jt] = mfma_f32(pt[tri(it, jt)][r], dov[it][r], du[jt]);
-#pragma unroll
-        for (int it = 0; it < 4; ++it)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int jt = 0; jt <= it; ++jt) R[jt] = mfma_f32(tt[tri(it, jt)][r], du[it][r], R[jt]);
+        for (int u = 0; u < 2; ++u) split(du[2 * u], du[2 * u + 1], f[u]);
+        blocks_times<2, true, NM>(tl, 0, 0, f[0], R, lane);
+        blocks_times<4, true, NM>(tl, 0, 1, f[1], R, lane);
         const float gc = sg[DC - 1];
 #pragma unroll
         for (int u = 0; u < HD / 16; ++u) G[u] *= gc;
+        const ChunkOf<T> vc = chunk_of((const T*)DV + ((b * L + t0) * H + h) * HD, (int64_t)H * HD, left);
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
             const f32x4_t b4 = *(const f32x4_t*)(sb + 16 * it + g4), gg = *(const f32x4_t*)(sg + 16 * it + g4);
@@ -501,13 +671,17 @@ __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict
                 const int i = 16 * it + g4 + r;
                 RS[(ci * DC + i) * HD + v] = R[it][r];
                 const float dv = b4[r] * R[it][r];
-                if (i < left) elem<T>::put(DV + ((b * L + t0 + i) * H + h) * HD + v, dv);
+                vc.put(i, v, dv);
                 dov[it][r] *= gg[r];
                 R[it][r] = -gg[r] * dv;
             }
         }
-        columns_times_tiles<HD>(qs, dov, G, m, g4);
-        columns_times_tiles<HD>(ks, R, G, m, g4);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) split(dov[2 * u], dov[2 * u + 1], f[u]);
+        columns_times<HD, NI>(qs, f, G, lane);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) split(R[2 * u], R[2 * u + 1], f[u]);
+        columns_times<HD, NI>(ks, f, G, lane);
     }
     if (DSTATE_IN != nullptr) {
 #pragma unroll
@@ -541,13 +715,15 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
     float* srv = (float*)(red + 4);
     float* fro = srv + DC;
     constexpr int NN = HD / 64;                    // column tiles of a wave
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g4 = (lane >> 4) * 4;
-    const int64_t ci = blockIdx.x;
-    const int64_t bh = ci / NC;
-    const int c = (int)(ci % NC), t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
-    const int64_t b = bh / H, h = bh % H;
-    rows_to_lds<HD, T, 256>(K, rk.at(b, L, t0, h, HD), rk.ld, left, ks, tid);
-    rows_to_lds<HD, T, 256>(Q, rq.at(b, L, t0, h, HD), rq.ld, left, qs, tid);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g4 = (lane >> 4) * 4;
+    int64_t b;
+    int h, c;
+    chunk_place(blockIdx.x, H, NC, b, h, c);
+    const int64_t ci = (b * H + h) * NC + c;
+    const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
+    const int64_t first = ((b * L + t0) * H + h) * HD, dense = (int64_t)H * HD;
+    rows_to_lds<HD, T>(chunk_of(K + rk.at(b, L, t0, h, HD), rk.ld, left), ks, tid);
+    rows_to_lds<HD, T>(chunk_of(Q + rq.at(b, L, t0, h, HD), rq.ld, left), qs, tid);
     if (tid < DC) {
         const int64_t at = (b * L + t0 + tid) * H + h;
         sa[tid] = tid < left ? ALPHA[at] : 1.0f;
@@ -555,16 +731,13 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
     }
     (&sdb[0][0])[tid] = 0.f;
     __syncthreads();
-    if (wave == 0) chunk_decays(sa, gt, lane);
-    if (wave == 1) sg[lane] = chunk_prefix(sa, lane);
+    if (wave == 0) chunk_decays(sa[lane], gt, lane);
+    if (wave == 1) sg[lane] = chunk_prefix(sa[lane], lane);
     __syncthreads();
     const float* ub = US + ci * DC * HD;
     const float* rb = RS + ci * DC * HD;
-    const T* dob = DO + ((b * L + t0) * H + h) * HD;
-    const int64_t dold = (int64_t)H * HD;
-    auto do4 = [&](int row, int col) -> f32x4_t {
-        return row < left ? load4(dob + (int64_t)row * dold + col) : (f32x4_t){0.f, 0.f, 0.f, 0.f};
-    };
+    const ChunkOf<T> doc = chunk_of(DO + first, dense, left), vc = chunk_of(V + rv.at(b, L, t0, h, HD), rv.ld, left);
+    auto do4 = [&](int row, int col) -> f32x4_t { return widen4(doc.raw(row, col)); };
     // the 64x64 matrices: lane holds column i, rows j = 4g..4g+3 of a tile
     for (int tile = wave; tile < TRI; tile += 4) {
         const int it = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, jt = tile - tri(it, 0);
@@ -614,7 +787,6 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
     const float* mb = MS + ci * HD * HD + wave * (HD / 4) + m;
     const float* gb = GS + ci * HD * HD + wave * (HD / 4) + m;
     float gm = 0.f, rdotv = 0.f;
-    const int64_t vrow = rv.at(b, L, t0, h, HD);
 #pragma unroll 1
     for (int u = 0; u < HD / 16; ++u) {
         const int col = 16 * u + g4;
@@ -636,8 +808,7 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
             }
         {
             const int row = 16 * wave + m;
-            f32x4_t vv = {0.f, 0.f, 0.f, 0.f};
-            if (row < left) vv = load4(V + vrow + (int64_t)row * rv.ld + col);
+            const f32x4_t vv = widen4(vc.raw(row, col));
             const f32x4_t rr = *(const f32x4_t*)(rb + row * HD + col);
 #pragma unroll
             for (int r = 0; r < 4; ++r) rdotv = fmaf(rr[r], vv[r], rdotv);
@@ -721,20 +892,17 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
                     Z[it][n] = mfma_f32(ae[it][r], bk[n][r], Z[it][n]);
                 }
     }
+    const ChunkOf<T> dqc = chunk_of((const T*)DQ + first, dense, left), dkc = chunk_of((const T*)DK + first, dense, left);
 #pragma unroll
     for (int it = 0; it < 4; ++it)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = 16 * it + g4 + r;
-            if (i < left) {
-                const int64_t at = ((b * L + t0 + i) * H + h) * HD + wave * (HD / 4) + m;
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int n = 0; n < NN; ++n) {
-                    elem<T>::put(DQ + at + 16 * n, X[it][n][r]);
-                    elem<T>::put(DK + at + 16 * n, Z[it][n][r]);
-                }
+            for (int n = 0; n < NN; ++n) {
+                const int i = 16 * it + g4 + r, col = wave * (HD / 4) + 16 * n + m;
+                dqc.put(i, col, X[it][n][r]);
+                dkc.put(i, col, Z[it][n][r]);
             }
-        }
     __syncthreads();                               // dm is free
     if (wave == 0) {
         const float ky = red[0][1][lane] + red[1][1][lane] + red[2][1][lane] + red[3][1][lane];
@@ -758,6 +926,18 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
     }
 }
 
+template <typename T> struct elem;
+template <> struct elem<float> {
+    static VA_DEVINL f32x4_t load4(const float* p) { return *(const f32x4_t*)p; }
+    static VA_DEVINL float get(const float* p) { return *p; }
+    static VA_DEVINL void put(float* p, float x) { *p = x; }
+};
+template <> struct elem<bf16_t> {
+    static VA_DEVINL f32x4_t load4(const bf16_t* p) { return widen4(*(const u32x2_t*)p); }
+    static VA_DEVINL float get(const bf16_t* p) { return bf16_to_f32(*p); }
+    static VA_DEVINL void put(bf16_t* p, float x) { *p = f32_to_bf16(x); }      // the output's own type: one rounding
+};
+
 // ---------------------------------------------------------------------------------------------------------------
 // One token: S <- a S + u k^T, u = b (v - a S k), o = S q = a (S_old q) + u (k.q).  The state is read and written once and
 // its rows are independent: HD/4 lanes hold a row (16 bytes each), the row's two dot products are summed across them.
@@ -771,7 +951,7 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const T* __restrict__ Q
     const int per = HD / rows_per_wg;
     const int64_t bh = blockIdx.x / per, b = bh / H, h = bh % H;
     const int row0 = (int)(blockIdx.x % per) * rows_per_wg;
-    const f32x4_t k4 = load4(K + b * ldk + h * HD + 4 * lane), q4 = load4(Q + b * ldq + h * HD + 4 * lane);
+    const f32x4_t k4 = elem<T>::load4(K + b * ldk + h * HD + 4 * lane), q4 = elem<T>::load4(Q + b * ldq + h * HD + 4 * lane);
     const float a = ALPHA[bh], bt = BETA[bh];
     float kq = 0.f;
 #pragma unroll
@@ -817,7 +997,7 @@ int delta_check(const char* who, const DeltaArgs& d) {
                  "%s: a row stride must be at least H * hd and a multiple of 4", who);
     VA_CHECK_ARG(((uintptr_t)d.q | (uintptr_t)d.k | (uintptr_t)d.v) % bytes == 0, "%s: misaligned operand", who);
     VA_CHECK_ARG(d.L < (1ll << 30) && d.H < (1ll << 20) && d.B < (1ll << 30) && d.B * d.H < (1ll << 24) &&
-                     d.B * d.H * d.chunks() < (1ll << 31) && d.ldq < (1ll << 30) && d.ldk < (1ll << 30) && d.ldv < (1ll << 30),
+                     d.B * d.H * d.chunks() < (1ll << 31) && d.ldq < (1 << 22) && d.ldk < (1 << 22) && d.ldv < (1 << 22),
                  "%s: problem too large", who);
     return VA_OK;
 }
@@ -836,21 +1016,29 @@ int reserve_lds(const char* who, const void* fn, int bytes) {
         if (rc__ != VA_OK) return rc__; \
     } while (0)
 
+// A workspace in pieces of 16 bytes.
+struct Pieces {
+    char* at;
+    template <typename E> E* take(int64_t n) {
+        E* p = (E*)at;
+        at += (n * (int64_t)sizeof(E) + 15) / 16 * 16;
+        return p;
+    }
+};
+
 template <int HD, typename T, bool GRAD>
-int launch_prep(const DeltaArgs& d, float* tf, float* tt, float* pf, float* gam, hipStream_t stream) {
-    constexpr int lds = (2 * DC * (HD + 4) + 2 * DC * SQ + DC * 20 + 2 * DC) * 4;
-    const auto fn = delta_prep_kernel<HD, T, GRAD>;
-    VA_TRY(reserve_lds("va_gated_delta", (const void*)fn, lds));
-    hipLaunchKernelGGL(fn, dim3((unsigned)(d.B * d.H * d.chunks())), dim3(256), lds, stream, (const T*)d.q, (const T*)d.k,
-                       Rows{d.ldq}, Rows{d.ldk}, d.alpha, d.beta, tf, tt, pf, gam, (int)d.L, (int)d.H, (int)d.chunks());
+int launch_prep(const DeltaArgs& d, bf16_t* tf, bf16_t* tt, bf16_t* pf, float* gam, hipStream_t stream) {
+    hipLaunchKernelGGL((delta_prep_kernel<HD, T, GRAD>), dim3((unsigned)(d.B * d.H * d.chunks())), dim3(256), 0, stream, (const T*)d.q,
+                       (const T*)d.k, Rows{d.ldq}, Rows{d.ldk}, d.alpha, d.beta, tf, tt, pf, gam, (int)d.L, (int)d.H,
+                       (int)d.chunks());
     VA_CHECK_LAUNCH("va_gated_delta (decays)");
     return VA_OK;
 }
 
 template <int HD, typename T, int W, bool OUT, bool SAVE>
-int launch_scan(const DeltaArgs& d, const float* tf, const float* pf, const float* gam, const float* state_in, void* out,
+int launch_scan(const DeltaArgs& d, const bf16_t* tf, const bf16_t* pf, const float* gam, const float* state_in, void* out,
                 float* state_out, float* us, float* ms, hipStream_t stream) {
-    constexpr int lds = ((OUT ? 2 : 1) * DC * (HD + 4) + 3 * DC) * 4;
+    constexpr int lds = ChunkRows<HD, T, W, OUT, parts<T>::MID, OUT ? parts<T>::OUT : 0>::LDS;
     const auto fn = delta_scan_kernel<HD, T, W, OUT, SAVE>;
     VA_TRY(reserve_lds("va_gated_delta", (const void*)fn, lds));
     hipLaunchKernelGGL(fn, dim3((unsigned)(d.B * d.H * (HD / 16 / W))), dim3(64 * W), lds, stream, (const T*)d.q, (const T*)d.k,
@@ -861,9 +1049,9 @@ int launch_scan(const DeltaArgs& d, const float* tf, const float* pf, const floa
 }
 
 template <int HD, typename T, int W>
-int launch_rscan(const DeltaArgs& d, const void* d_out, const float* tt, const float* pt, const float* gam, const float* d_state,
+int launch_rscan(const DeltaArgs& d, const void* d_out, const bf16_t* tt, const bf16_t* pt, const float* gam, const float* d_state,
                  void* dv, float* d_state_in, float* rs, float* gs, hipStream_t stream) {
-    constexpr int lds = (2 * DC * (HD + 4) + 3 * DC) * 4;
+    constexpr int lds = ChunkRows<HD, T, W, true, parts<T>::MID, parts<T>::MID>::LDS;
     const auto fn = delta_rscan_kernel<HD, T, W>;
     VA_TRY(reserve_lds("va_gated_delta_bwd", (const void*)fn, lds));
     hipLaunchKernelGGL(fn, dim3((unsigned)(d.B * d.H * (HD / 16 / W))), dim3(64 * W), lds, stream, (const T*)d.q, (const T*)d.k,
@@ -877,12 +1065,18 @@ int launch_rscan(const DeltaArgs& d, const void* d_out, const float* tt, const f
 // rows.  Few heads are spread over as many CUs as there are pairs of waves, many heads keep all columns together.
 int scan_waves(int64_t heads, int hd) { return heads * (hd / 16) >= 8 * 256 ? hd / 16 : 2; }
 
-constexpr int64_t FWD_CHUNK_FLOATS = 2 * TRI * FRAG + 2 * DC;
+// bytes of one chunk's share of a workspace
+constexpr int64_t OPERAND_BYTES = BLK * BFRAG * 2;
+int64_t fwd_chunk_bytes() { return 6 * OPERAND_BYTES + 2 * DC * 4; }
+int64_t bwd_chunk_bytes(int64_t hd) { return 9 * OPERAND_BYTES + 2 * DC * 4 + 2 * DC * hd * 4 + 2 * hd * hd * 4; }
 
 template <int HD, typename T>
 int delta_fwd(const DeltaArgs& d, const float* state_in, void* out, float* state_out, float* ws, hipStream_t stream) {
     const int64_t n = d.B * d.H * d.chunks();
-    float *tf = ws, *pf = tf + n * TRI * FRAG, *gam = pf + n * TRI * FRAG;
+    Pieces w = {(char*)ws};
+    bf16_t* tf = w.take<bf16_t>(n * BLK * BFRAG * parts<T>::MID);
+    bf16_t* pf = w.take<bf16_t>(n * BLK * BFRAG * parts<T>::OUT);
+    float* gam = w.take<float>(n * 2 * DC);
     VA_TRY((launch_prep<HD, T, false>(d, tf, nullptr, pf, gam, stream)));
     if (scan_waves(d.B * d.H, HD) == 2)
         return launch_scan<HD, T, 2, true, false>(d, tf, pf, gam, state_in, out, state_out, nullptr, nullptr, stream);
@@ -892,9 +1086,11 @@ int delta_fwd(const DeltaArgs& d, const float* state_in, void* out, float* state
 template <int HD, typename T>
 int delta_bwd(const DeltaArgs& d, const void* d_out, const float* d_state, const float* state_in, void* dq, void* dk, void* dv,
               float* dalpha, float* dbeta, float* d_state_in, float* ws, hipStream_t stream) {
-    const int64_t n = d.B * d.H * d.chunks();
-    float *tf = ws, *tt = tf + n * TRI * FRAG, *pt = tt + n * TRI * FRAG, *gam = pt + n * TRI * FRAG;
-    float *us = gam + n * 2 * DC, *rs = us + n * DC * HD, *ms = rs + n * DC * HD, *gs = ms + n * HD * HD;
+    const int64_t n = d.B * d.H * d.chunks(), ops = n * BLK * BFRAG * parts<T>::MID;
+    Pieces w = {(char*)ws};
+    bf16_t *tf = w.take<bf16_t>(ops), *tt = w.take<bf16_t>(ops), *pt = w.take<bf16_t>(ops);
+    float *gam = w.take<float>(n * 2 * DC), *us = w.take<float>(n * DC * HD), *rs = w.take<float>(n * DC * HD);
+    float *ms = w.take<float>(n * HD * HD), *gs = w.take<float>(n * HD * HD);
     VA_TRY((launch_prep<HD, T, true>(d, tf, tt, pt, gam, stream)));
     if (scan_waves(d.B * d.H, HD) == 2) {
         VA_TRY((launch_scan<HD, T, 2, false, true>(d, tf, nullptr, gam, state_in, nullptr, nullptr, us, ms, stream)));
@@ -917,12 +1113,12 @@ int delta_bwd(const DeltaArgs& d, const void* d_out, const float* d_state, const
 
 extern "C" int64_t va_gated_delta_fwd_workspace_floats(int64_t B, int64_t L, int64_t H, int64_t hd) {
     if (B <= 0 || L <= 0 || H <= 0 || (hd != 64 && hd != 128)) return 0;
-    return B * H * ((L + DC - 1) / DC) * FWD_CHUNK_FLOATS;
+    return B * H * ((L + DC - 1) / DC) * fwd_chunk_bytes() / 4;
 }
 
 extern "C" int64_t va_gated_delta_bwd_workspace_floats(int64_t B, int64_t L, int64_t H, int64_t hd) {
     if (B <= 0 || L <= 0 || H <= 0 || (hd != 64 && hd != 128)) return 0;
-    return B * H * ((L + DC - 1) / DC) * (3 * TRI * FRAG + 2 * DC + 2 * DC * hd + 2 * hd * hd);
+    return B * H * ((L + DC - 1) / DC) * bwd_chunk_bytes(hd) / 4;
 }
 
 extern "C" int va_gated_delta_fwd(const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv, int is_bf16,

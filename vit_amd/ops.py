@@ -17,7 +17,12 @@ BF16, F32 = torch.bfloat16, torch.float32
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)     # the binding itself: this runs per tensor
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream() -> int:
+    if _raw_stream is not None:                      # the handle without a Stream object around it: this runs per call
+        return _raw_stream(_current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -26,15 +31,16 @@ def _p(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _need(t: torch.Tensor, dtype, name: str, inner_contig: bool = True):
-    if not t.is_cuda:
+    device = t.get_device()
+    if device < 0:
         raise _lib.VitAmdError(f"{name}: tensor must live on a HIP device (vit_amd has no CPU path)")
-    if t.device.index != _current_device():
+    if device != _current_device():
         # kernels are launched on the CURRENT device's stream: a tensor of another device would be a wild pointer there
         raise _lib.VitAmdError(f"{name}: tensor is on {t.device} but the current device is cuda:{_current_device()}; "
                                "wrap the call in torch.cuda.device(tensor.device) (VideoViTEncoder.forward does)")
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if inner_contig and t.dim() >= 1 and t.stride(-1) != 1:
+    if inner_contig and not t.is_contiguous() and t.stride(-1) != 1:
         raise ValueError(f"{name}: innermost dimension must be contiguous")
 
 
@@ -553,10 +559,12 @@ def _heads_ld(t: torch.Tensor, name: str) -> int:
     """Elements between the token rows of q / k / v [B, L, H, hd] (or [B, H, hd]): heads lie side by side in a row, rows
     one constant stride apart over the whole batch (a contiguous tensor, or a column block of a wider matrix)."""
     lead, H, hd = t.shape[:-2], t.shape[-2], t.shape[-1]
+    if t.is_contiguous():
+        return H * hd
     if t.stride(-1) != 1 or (H > 1 and t.stride(-2) != hd):
         raise ValueError(f"{name}: the heads of a token must lie side by side")
     ld = None
-    for size, stride, rows in zip(reversed(lead), reversed(t.stride()[:-2]), ([1, lead[-1]] if len(lead) > 1 else [1])):
+    for size, stride, rows in zip(reversed(lead), reversed(t.stride()[:-2]), (1, lead[-1])):
         if size > 1:
             if stride % rows or (ld is not None and stride != rows * ld):
                 raise ValueError(f"{name}: token rows must be one constant stride apart")
@@ -565,21 +573,22 @@ def _heads_ld(t: torch.Tensor, name: str) -> int:
 
 
 def _delta_operands(who: str, q, k, v, alpha, beta, state, lead: int):
-    if q.dtype not in (F32, BF16):
+    dtype, shape = q.dtype, q.shape
+    if dtype is not F32 and dtype is not BF16:
         raise TypeError(f"{who}: q, k, v must be f32 or bf16")
-    if q.dim() != lead + 2:
+    if len(shape) != lead + 2:
         raise ValueError(f"{who}: q must have {lead + 2} dimensions")
-    if 0 in q.shape:
+    if q.numel() == 0:
         raise ValueError(f"{who}: empty problem")
     for name, x in (("q", q), ("k", k), ("v", v)):
-        _need(x, q.dtype, name)
-        if x.shape != q.shape:
+        _need(x, dtype, name)
+        if x.shape != shape:
             raise ValueError(f"{who}: q, k, v must share one shape")
     for name, x in (("alpha", alpha), ("beta", beta)):
         _need(x, F32, name)
-        if x.shape != q.shape[:-1] or not x.is_contiguous():
-            raise ValueError(f"{who}: {name} must be contiguous {tuple(q.shape[:-1])}")
-    B, H, hd = q.shape[0], q.shape[-2], q.shape[-1]
+        if x.shape != shape[:-1] or not x.is_contiguous():
+            raise ValueError(f"{who}: {name} must be contiguous {tuple(shape[:-1])}")
+    B, H, hd = shape[0], shape[-2], shape[-1]
     if state is not None:
         _need(state, F32, "state")
         if tuple(state.shape) != (B, H, hd, hd) or not state.is_contiguous():
