@@ -118,10 +118,10 @@ VA_DEVINL void split(f32x4_t a, f32x4_t b, bf16x8_t (&out)[N]) {
         out[n] = __builtin_bit_cast(bf16x8_t, w);
     }
 }
-// acc[x] += a[x] * b from their parts, every pair whose product is above 2^-24 of the whole; independent accumulators follow
-// each other
-template <int X, int NA, int NB>
-VA_DEVINL void mfma_parts_of(const bf16x8_t (&a)[X][NA], const bf16x8_t (&b)[NB], f32x4_t* acc) {
+// acc[c][first + x] += a[x] * b[c] from their parts, every pair whose product is above 2^-24 of the whole; independent
+// accumulators follow each other
+template <int X, int NA, int NB, int CG, int N>
+VA_DEVINL void mfma_parts(const bf16x8_t (&a)[X][NA], const bf16x8_t (&b)[CG][NB], f32x4_t (&acc)[CG][N], int first) {
     constexpr int KEEP = NA > NB ? NA : NB;
 #pragma unroll
     for (int i = NA - 1; i >= 0; --i)
@@ -129,7 +129,9 @@ VA_DEVINL void mfma_parts_of(const bf16x8_t (&a)[X][NA], const bf16x8_t (&b)[NB]
         for (int j = NB - 1; j >= 0; --j)
             if (i + j < KEEP) {
 #pragma unroll
-                for (int x = 0; x < X; ++x) acc[x] = mfma16(a[x][i], b[j], acc[x]);
+                for (int x = 0; x < X; ++x)
+#pragma unroll
+                    for (int c = 0; c < CG; ++c) acc[c][first + x] = mfma16(a[x][i], b[c][j], acc[c][first + x]);
             }
 }
 // operand blocks: (row tile it, columns 32u..) of a lower triangle, and of an upper one
@@ -140,13 +142,13 @@ VA_DEVINL void load_block(const char* base, int block, int lane, bf16x8_t (&out)
 #pragma unroll
     for (int n = 0; n < N; ++n) out[n] = *(const bf16x8_t*)(base + (block * N + n) * BFRAG * 2 + lane * 16);
 }
-// acc[first..] += (row tiles first..first + X - 1, column block u) of an operand in LDS times b
-template <int X, bool UP, int NA, int NB>
-VA_DEVINL void blocks_times(const char* base, int first, int u, const bf16x8_t (&b)[NB], f32x4_t* acc, int lane) {
+// acc[c][first..] += (row tiles first..first + X - 1, column block u) of an operand in LDS times b
+template <int X, bool UP, int NA, int NB, int CG>
+VA_DEVINL void blocks_times(const char* base, int first, int u, const bf16x8_t (&b)[CG][NB], f32x4_t (&acc)[CG][4], int lane) {
     bf16x8_t a[X][NA];
 #pragma unroll
     for (int x = 0; x < X; ++x) load_block(base, UP ? up_block(first + x, u) : low_block(first + x, u), lane, a[x]);
-    mfma_parts_of<X>(a, b, acc + first);
+    mfma_parts(a, b, acc, first);
 }
 template <int N>
 VA_DEVINL void store_block(bf16_t* base, int block, int lane, const bf16x8_t (&v)[N]) {
@@ -452,34 +454,36 @@ struct ChunkRows {
     }
 };
 
-// acc[ct] += X^T B for all HD/16 column tiles of X, B in parts
-template <int HD, int NX, int NB>
-VA_DEVINL void columns_times(const char* x, const bf16x8_t (&bt)[2][NB], f32x4_t* acc, int lane) {
+// acc[c][ct] += X^T B for all HD/16 column tiles of X, B (token blocks u) in parts
+template <int HD, int NX, int NB, int CG>
+VA_DEVINL void columns_times(const char* x, const bf16x8_t (&b0)[CG][NB], const bf16x8_t (&b1)[CG][NB], f32x4_t (&acc)[CG][HD / 16],
+                             int lane) {
 #pragma unroll
-    for (int ct = 0; ct < HD / 16; ct += 2)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            bf16x8_t a[2][NX];
-            col_frag<HD>(x, ct, u, lane, a[0]);
-            col_frag<HD>(x, ct + 1, u, lane, a[1]);
-            mfma_parts_of<2>(a, bt[u], acc + ct);
-        }
+    for (int ct = 0; ct < HD / 16; ct += 2) {
+        bf16x8_t a[2][NX];
+        col_frag<HD>(x, ct, 0, lane, a[0]);
+        col_frag<HD>(x, ct + 1, 0, lane, a[1]);
+        mfma_parts(a, b0, acc, ct);
+        col_frag<HD>(x, ct, 1, lane, a[0]);
+        col_frag<HD>(x, ct + 1, 1, lane, a[1]);
+        mfma_parts(a, b1, acc, ct);
+    }
 }
-// acc[it] += rows of X times B (tiles it, column block u)
-template <int HD, int NX, int NB>
-VA_DEVINL void rows_times(const char* x, int u, const bf16x8_t (&bt)[NB], f32x4_t* acc, int m, int g) {
+// acc[c][it] += rows of X times B (column block u)
+template <int HD, int NX, int NB, int CG>
+VA_DEVINL void rows_times(const char* x, int u, const bf16x8_t (&b)[CG][NB], f32x4_t (&acc)[CG][4], int m, int g) {
     bf16x8_t a[4][NX];
 #pragma unroll
     for (int it = 0; it < 4; ++it) row_frag<HD>(x, it, u, m, g, a[it]);
-    mfma_parts_of<4>(a, bt, acc);
+    mfma_parts(a, b, acc, 0);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// The sequential part.  A wave owns 16 columns (values of the head) of the state for the whole sequence: M in HD/16
+// The sequential part.  A wave owns 16 CG columns (values of the head) of the state for the whole sequence: M in CG * HD/16
 // accumulator tiles; W waves share a chunk's K, Q, T and P through LDS.  K and Q of the next chunk are requested half-way
 // through the current one, T and P of a chunk arrive while its products with M are formed.
 // OUT: writes o.  SAVE: writes U and every chunk's starting state (rows of S) for the gradient.
-template <int HD, typename T, int W, bool OUT, bool SAVE>
+template <int HD, typename T, int W, int CG, bool OUT, bool SAVE>
 __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                                                             Rows rq, Rows rk, Rows rv, const float* __restrict__ BETA,
                                                             const bf16_t* __restrict__ TF, const bf16_t* __restrict__ PF,
@@ -492,21 +496,23 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
     const char *ks = lds, *qs = lds + CR::MATRIX;
     char *tl = lds + CR::A_AT, *pl = lds + CR::B_AT;
     const float *sb = (const float*)(lds + CR::F_AT), *sg = sb + DC, *se = sg + DC;
-    constexpr int GROUPS = HD / 16 / W;
+    constexpr int GROUPS = HD / 16 / (W * CG);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4, g4 = g * 4;
     const int wid = xcd_remap(blockIdx.x, gridDim.x);
     const int64_t bh = wid / GROUPS, b = bh / H, h = bh % H;
-    const int v = ((wid % GROUPS) * W + wave) * 16 + m;
+    const int v = ((wid % GROUPS) * W + wave) * 16 * CG + m;      // and v + 16 in the second group
     const T* vb = V + rv.at(b, L, 0, h, HD);
     CR cr;
     cr.k = K + rk.at(b, L, 0, h, HD), cr.q = Q + rq.at(b, L, 0, h, HD), cr.ldk = rk.ld, cr.ldq = rq.ld;
     cr.beta = BETA + b * L * H + h, cr.gam = GAM + bh * NC * 2 * DC, cr.L = L, cr.H = H, cr.tid = tid;
-    f32x4_t M[HD / 16];
+    f32x4_t M[CG][HD / 16];
 #pragma unroll
-    for (int u = 0; u < HD / 16; ++u) {
-        M[u] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-        if (STATE_IN != nullptr) M[u] = *(const f32x4_t*)(STATE_IN + (bh * HD + v) * HD + 16 * u + g4);
-    }
+    for (int x = 0; x < CG; ++x)
+#pragma unroll
+        for (int u = 0; u < HD / 16; ++u) {
+            M[x][u] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            if (STATE_IN != nullptr) M[x][u] = *(const f32x4_t*)(STATE_IN + (bh * HD + v + 16 * x) * HD + 16 * u + g4);
+        }
     cr.request(0, NC);
     for (int c = 0; c < NC; ++c) {
         const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
@@ -515,84 +521,107 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
         cr.place(lds);
         to_lds<CR::A_BYTES, W>(TF + ci * BLK * NM * BFRAG, tl, wave, lane);
         if (OUT) to_lds<CR::B_BYTES, W>(PF + ci * BLK * NO * BFRAG, pl, wave, lane);
-        f32x4_t vv[4];                            // this chunk's v column, rows in accumulator order
+        f32x4_t vv[CG][4];                        // this chunk's v columns, rows in accumulator order
         const ChunkOf<T> vc = chunk_of(vb + (int64_t)t0 * rv.ld, rv.ld, left);
 #pragma unroll
-        for (int it = 0; it < 4; ++it)
+        for (int x = 0; x < CG; ++x)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) vv[it][r] = vc.get(16 * it + g4 + r, v);
+            for (int it = 0; it < 4; ++it)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vv[x][it][r] = vc.get(16 * it + g4 + r, v + 16 * x);
         lds_barrier();
-        if (SAVE) {
+        f32x4_t rhs[CG][4], o[CG][4], U[CG][4];
 #pragma unroll
-            for (int u = 0; u < HD / 16; ++u) *(f32x4_t*)(MS + (ci * HD + v) * HD + 16 * u + g4) = M[u];
+        for (int x = 0; x < CG; ++x) {
+            if (SAVE) {
+#pragma unroll
+                for (int u = 0; u < HD / 16; ++u) *(f32x4_t*)(MS + (ci * HD + v + 16 * x) * HD + 16 * u + g4) = M[x][u];
+            }
+#pragma unroll
+            for (int it = 0; it < 4; ++it) rhs[x][it] = o[x][it] = U[x][it] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
         }
-        f32x4_t rhs[4], o[4], U[4];
-#pragma unroll
-        for (int it = 0; it < 4; ++it) rhs[it] = o[it] = U[it] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < HD / 32; ++u) {
-            bf16x8_t mf[NM], mo[NO];
-            split(M[2 * u], M[2 * u + 1], mf);
-            rows_times<HD, NI>(ks, u, mf, rhs, m, g);
-            if (OUT) {
+            bf16x8_t mf[CG][NM], mo[CG][NO];
 #pragma unroll
-                for (int n = 0; n < NO; ++n) mo[n] = mf[n];
-                rows_times<HD, NI>(qs, u, mo, o, m, g);
+            for (int x = 0; x < CG; ++x) {
+                split(M[x][2 * u], M[x][2 * u + 1], mf[x]);
+#pragma unroll
+                for (int n = 0; n < NO; ++n) mo[x][n] = mf[x][n];
             }
+            rows_times<HD, NI>(ks, u, mf, rhs, m, g);
+            if (OUT) rows_times<HD, NI>(qs, u, mo, o, m, g);
         }
+        bf16x8_t f0[CG][NM], f1[CG][NM];
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
             const f32x4_t b4 = *(const f32x4_t*)(sb + 16 * it + g4), gg = *(const f32x4_t*)(sg + 16 * it + g4);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                rhs[it][r] = b4[r] * (vv[it][r] - gg[r] * rhs[it][r]);
-                o[it][r] *= gg[r];
-            }
-        }
-        bf16x8_t f[2][NM];
+            for (int x = 0; x < CG; ++x)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) split(rhs[2 * u], rhs[2 * u + 1], f[u]);
+                for (int r = 0; r < 4; ++r) {
+                    rhs[x][it][r] = b4[r] * (vv[x][it][r] - gg[r] * rhs[x][it][r]);
+                    o[x][it][r] *= gg[r];
+                }
+        }
+#pragma unroll
+        for (int x = 0; x < CG; ++x) {
+            split(rhs[x][0], rhs[x][1], f0[x]);
+            split(rhs[x][2], rhs[x][3], f1[x]);
+        }
         wait_vm0();
         __syncthreads();                          // T and P are there
         cr.request(c + 1, NC);
-        blocks_times<4, false, NM>(tl, 0, 0, f[0], U, lane);
-        blocks_times<2, false, NM>(tl, 2, 1, f[1], U, lane);
+        blocks_times<4, false, NM>(tl, 0, 0, f0, U, lane);
+        blocks_times<2, false, NM>(tl, 2, 1, f1, U, lane);
         if (SAVE) {
 #pragma unroll
-            for (int it = 0; it < 4; ++it)
+            for (int x = 0; x < CG; ++x)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) US[(ci * DC + 16 * it + g4 + r) * HD + v] = U[it][r];
+                for (int it = 0; it < 4; ++it)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) US[(ci * DC + 16 * it + g4 + r) * HD + v + 16 * x] = U[x][it][r];
         }
         if (OUT) {
-            bf16x8_t uf[2][NO];
+            bf16x8_t u0[CG][NO], u1[CG][NO];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) split(U[2 * u], U[2 * u + 1], uf[u]);
-            blocks_times<4, false, NO>(pl, 0, 0, uf[0], o, lane);
-            blocks_times<2, false, NO>(pl, 2, 1, uf[1], o, lane);
+            for (int x = 0; x < CG; ++x) {
+                split(U[x][0], U[x][1], u0[x]);
+                split(U[x][2], U[x][3], u1[x]);
+            }
+            blocks_times<4, false, NO>(pl, 0, 0, u0, o, lane);
+            blocks_times<2, false, NO>(pl, 2, 1, u1, o, lane);
             const ChunkOf<T> oc = chunk_of((const T*)O + ((b * L + t0) * H + h) * HD, (int64_t)H * HD, left);
 #pragma unroll
-            for (int it = 0; it < 4; ++it)
+            for (int x = 0; x < CG; ++x)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) oc.put(16 * it + g4 + r, v, o[it][r]);
+                for (int it = 0; it < 4; ++it)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) oc.put(16 * it + g4 + r, v + 16 * x, o[x][it][r]);
         }
         const float gc = sg[DC - 1];
 #pragma unroll
-        for (int u = 0; u < HD / 16; ++u) M[u] *= gc;
+        for (int x = 0; x < CG; ++x) {
 #pragma unroll
-        for (int it = 0; it < 4; ++it) U[it] *= *(const f32x4_t*)(se + 16 * it + g4);
+            for (int u = 0; u < HD / 16; ++u) M[x][u] *= gc;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) split(U[2 * u], U[2 * u + 1], f[u]);
-        columns_times<HD, NI>(ks, f, M, lane);
+            for (int it = 0; it < 4; ++it) U[x][it] *= *(const f32x4_t*)(se + 16 * it + g4);
+            split(U[x][0], U[x][1], f0[x]);
+            split(U[x][2], U[x][3], f1[x]);
+        }
+        columns_times<HD, NI>(ks, f0, f1, M, lane);
     }
     if (STATE_OUT != nullptr) {
 #pragma unroll
-        for (int u = 0; u < HD / 16; ++u) *(f32x4_t*)(STATE_OUT + (bh * HD + v) * HD + 16 * u + g4) = M[u];
+        for (int x = 0; x < CG; ++x)
+#pragma unroll
+            for (int u = 0; u < HD / 16; ++u) *(f32x4_t*)(STATE_OUT + (bh * HD + v + 16 * x) * HD + 16 * u + g4) = M[x][u];
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // The same walk backwards for G = dL/dM: writes every chunk's G (at its end, rows of dS), R and dv.
-template <int HD, typename T, int W>
+template <int HD, typename T, int W, int CG>
 __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict__ Q, const T* __restrict__ K, Rows rq, Rows rk,
                                                              const T* __restrict__ DO, const float* __restrict__ BETA,
                                                              const bf16_t* __restrict__ TT, const bf16_t* __restrict__ PT,
@@ -605,20 +634,22 @@ __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict
     const char *ks = lds, *qs = lds + CR::MATRIX;
     char *pl = lds + CR::A_AT, *tl = lds + CR::B_AT;
     const float *sb = (const float*)(lds + CR::F_AT), *sg = sb + DC, *se = sg + DC;
-    constexpr int GROUPS = HD / 16 / W;
+    constexpr int GROUPS = HD / 16 / (W * CG);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4, g4 = g * 4;
     const int wid = xcd_remap(blockIdx.x, gridDim.x);
     const int64_t bh = wid / GROUPS, b = bh / H, h = bh % H;
-    const int v = ((wid % GROUPS) * W + wave) * 16 + m;
+    const int v = ((wid % GROUPS) * W + wave) * 16 * CG + m;
     CR cr;
     cr.k = K + rk.at(b, L, 0, h, HD), cr.q = Q + rq.at(b, L, 0, h, HD), cr.ldk = rk.ld, cr.ldq = rq.ld;
     cr.beta = BETA + b * L * H + h, cr.gam = GAM + bh * NC * 2 * DC, cr.L = L, cr.H = H, cr.tid = tid;
-    f32x4_t G[HD / 16];
+    f32x4_t G[CG][HD / 16];
 #pragma unroll
-    for (int u = 0; u < HD / 16; ++u) {
-        G[u] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-        if (DSTATE != nullptr) G[u] = *(const f32x4_t*)(DSTATE + (bh * HD + v) * HD + 16 * u + g4);
-    }
+    for (int x = 0; x < CG; ++x)
+#pragma unroll
+        for (int u = 0; u < HD / 16; ++u) {
+            G[x][u] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            if (DSTATE != nullptr) G[x][u] = *(const f32x4_t*)(DSTATE + (bh * HD + v + 16 * x) * HD + 16 * u + g4);
+        }
     cr.request(NC - 1, NC);
     for (int c = NC - 1; c >= 0; --c) {
         const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
@@ -627,65 +658,85 @@ __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict
         cr.place(lds);
         to_lds<CR::A_BYTES, W>(PT + ci * BLK * NM * BFRAG, pl, wave, lane);
         to_lds<CR::B_BYTES, W>(TT + ci * BLK * NM * BFRAG, tl, wave, lane);
-        f32x4_t dov[4];
+        f32x4_t dov[CG][4];
         const ChunkOf<T> oc = chunk_of(DO + ((b * L + t0) * H + h) * HD, (int64_t)H * HD, left);
 #pragma unroll
-        for (int it = 0; it < 4; ++it)
+        for (int x = 0; x < CG; ++x)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) dov[it][r] = oc.get(16 * it + g4 + r, v);
+            for (int it = 0; it < 4; ++it)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dov[x][it][r] = oc.get(16 * it + g4 + r, v + 16 * x);
         lds_barrier();
+        f32x4_t du[CG][4], R[CG][4];
 #pragma unroll
-        for (int u = 0; u < HD / 16; ++u) *(f32x4_t*)(GS + (ci * HD + v) * HD + 16 * u + g4) = G[u];
-        f32x4_t du[4], R[4];
+        for (int x = 0; x < CG; ++x) {
 #pragma unroll
-        for (int it = 0; it < 4; ++it) du[it] = R[it] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            for (int u = 0; u < HD / 16; ++u) *(f32x4_t*)(GS + (ci * HD + v + 16 * x) * HD + 16 * u + g4) = G[x][u];
 #pragma unroll
-        for (int u = 0; u < HD / 32; ++u) {
-            bf16x8_t gf[NM];
-            split(G[2 * u], G[2 * u + 1], gf);
-            rows_times<HD, NI>(ks, u, gf, du, m, g);
+            for (int it = 0; it < 4; ++it) du[x][it] = R[x][it] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
         }
 #pragma unroll
-        for (int it = 0; it < 4; ++it) du[it] *= *(const f32x4_t*)(se + 16 * it + g4);
-        bf16x8_t of[2][NI], f[2][NM];
+        for (int u = 0; u < HD / 32; ++u) {
+            bf16x8_t gf[CG][NM];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) split(dov[2 * u], dov[2 * u + 1], of[u]);
+            for (int x = 0; x < CG; ++x) split(G[x][2 * u], G[x][2 * u + 1], gf[x]);
+            rows_times<HD, NI>(ks, u, gf, du, m, g);
+        }
+        bf16x8_t o0[CG][NI], o1[CG][NI], f0[CG][NM], f1[CG][NM];
+#pragma unroll
+        for (int x = 0; x < CG; ++x) {
+#pragma unroll
+            for (int it = 0; it < 4; ++it) du[x][it] *= *(const f32x4_t*)(se + 16 * it + g4);
+            split(dov[x][0], dov[x][1], o0[x]);
+            split(dov[x][2], dov[x][3], o1[x]);
+        }
         wait_vm0();
         __syncthreads();                          // P^T and T^T are there
         cr.request(c - 1, NC);
-        blocks_times<2, true, NM>(pl, 0, 0, of[0], du, lane);
-        blocks_times<4, true, NM>(pl, 0, 1, of[1], du, lane);
+        blocks_times<2, true, NM>(pl, 0, 0, o0, du, lane);
+        blocks_times<4, true, NM>(pl, 0, 1, o1, du, lane);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) split(du[2 * u], du[2 * u + 1], f[u]);
-        blocks_times<2, true, NM>(tl, 0, 0, f[0], R, lane);
-        blocks_times<4, true, NM>(tl, 0, 1, f[1], R, lane);
+        for (int x = 0; x < CG; ++x) {
+            split(du[x][0], du[x][1], f0[x]);
+            split(du[x][2], du[x][3], f1[x]);
+        }
+        blocks_times<2, true, NM>(tl, 0, 0, f0, R, lane);
+        blocks_times<4, true, NM>(tl, 0, 1, f1, R, lane);
         const float gc = sg[DC - 1];
-#pragma unroll
-        for (int u = 0; u < HD / 16; ++u) G[u] *= gc;
         const ChunkOf<T> vc = chunk_of((const T*)DV + ((b * L + t0) * H + h) * HD, (int64_t)H * HD, left);
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-            const f32x4_t b4 = *(const f32x4_t*)(sb + 16 * it + g4), gg = *(const f32x4_t*)(sg + 16 * it + g4);
+        for (int x = 0; x < CG; ++x) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * it + g4 + r;
-                RS[(ci * DC + i) * HD + v] = R[it][r];
-                const float dv = b4[r] * R[it][r];
-                vc.put(i, v, dv);
-                dov[it][r] *= gg[r];
-                R[it][r] = -gg[r] * dv;
+            for (int u = 0; u < HD / 16; ++u) G[x][u] *= gc;
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                const f32x4_t b4 = *(const f32x4_t*)(sb + 16 * it + g4), gg = *(const f32x4_t*)(sg + 16 * it + g4);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = 16 * it + g4 + r;
+                    RS[(ci * DC + i) * HD + v + 16 * x] = R[x][it][r];
+                    const float dv = b4[r] * R[x][it][r];
+                    vc.put(i, v + 16 * x, dv);
+                    dov[x][it][r] *= gg[r];
+                    R[x][it][r] = -gg[r] * dv;
+                }
             }
+            split(dov[x][0], dov[x][1], f0[x]);
+            split(dov[x][2], dov[x][3], f1[x]);
         }
+        columns_times<HD, NI>(qs, f0, f1, G, lane);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) split(dov[2 * u], dov[2 * u + 1], f[u]);
-        columns_times<HD, NI>(qs, f, G, lane);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) split(R[2 * u], R[2 * u + 1], f[u]);
-        columns_times<HD, NI>(ks, f, G, lane);
+        for (int x = 0; x < CG; ++x) {
+            split(R[x][0], R[x][1], f0[x]);
+            split(R[x][2], R[x][3], f1[x]);
+        }
+        columns_times<HD, NI>(ks, f0, f1, G, lane);
     }
     if (DSTATE_IN != nullptr) {
 #pragma unroll
-        for (int u = 0; u < HD / 16; ++u) *(f32x4_t*)(DSTATE_IN + (bh * HD + v) * HD + 16 * u + g4) = G[u];
+        for (int x = 0; x < CG; ++x)
+#pragma unroll
+            for (int u = 0; u < HD / 16; ++u) *(f32x4_t*)(DSTATE_IN + (bh * HD + v + 16 * x) * HD + 16 * u + g4) = G[x][u];
     }
 }
 
@@ -705,7 +756,7 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
     float(*qs)[HD + 4] = ks + DC;
     float(*gt)[SQ] = (float(*)[SQ])(qs + DC);      // decays, [j][i]
     float(*dg)[SQ] = gt + DC;                      // gradients of the decays, [j][i]
-    float(*dm)[SQ] = dg + DC;                      // dP o g, [i][j]; later the terms of da
+    float(*dm)[SQ] = dg + DC;                      // dP o g, [i][j]
     float(*es)[SQ] = dm + DC;                      // E + E^T
     float* sa = (float*)(es + DC);
     float* sb = sa + DC;
@@ -714,6 +765,7 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
     float(*red)[3][DC] = (float(*)[3][DC])(sdb + 4);   // [wave][q.X, k.Y, k.Z][i]
     float* srv = (float*)(red + 4);
     float* fro = srv + DC;
+    float *sky = fro + 4, *sdg = sky + DC;         // k_i.Y_i, d(g_i)
     constexpr int NN = HD / 64;                    // column tiles of a wave
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g4 = (lane >> 4) * 4;
     int64_t b;
@@ -743,7 +795,7 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
         const int it = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, jt = tile - tri(it, 0);
         const int i = 16 * it + m, jr = 16 * jt + m;
         f32x4_t qk = {0.f, 0.f, 0.f, 0.f}, kk = qk, dp = qk, ru = qk;
-#pragma unroll 4
+#pragma unroll
         for (int u = 0; u < HD / 16; ++u) {
             const int col = 16 * u + g4;
             const f32x4_t kj = *(const f32x4_t*)&ks[jr][col], qi = *(const f32x4_t*)&qs[i][col],
@@ -787,44 +839,53 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
     const float* mb = MS + ci * HD * HD + wave * (HD / 4) + m;
     const float* gb = GS + ci * HD * HD + wave * (HD / 4) + m;
     float gm = 0.f, rdotv = 0.f;
-#pragma unroll 1
-    for (int u = 0; u < HD / 16; ++u) {
+    struct Operands {
+        f32x4_t o[4], r[4], u[4], rr, vv;
+        float m[NN][4], g[NN][4];
+    };
+    auto load = [&](Operands& x, int u) {
         const int col = 16 * u + g4;
-        f32x4_t ao[4], ar[4], au[4];
-        float bm[NN][4], bg[NN][4];
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
             const int row = 16 * it + m;
-            ao[it] = do4(row, col);
-            ar[it] = *(const f32x4_t*)(rb + row * HD + col);
-            au[it] = *(const f32x4_t*)(ub + row * HD + col);
+            x.o[it] = do4(row, col);
+            x.r[it] = *(const f32x4_t*)(rb + row * HD + col);
+            x.u[it] = *(const f32x4_t*)(ub + row * HD + col);
         }
 #pragma unroll
         for (int n = 0; n < NN; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                bm[n][r] = mb[(col + r) * HD + 16 * n];
-                bg[n][r] = gb[(col + r) * HD + 16 * n];
+                x.m[n][r] = mb[(col + r) * HD + 16 * n];
+                x.g[n][r] = gb[(col + r) * HD + 16 * n];
             }
-        {
-            const int row = 16 * wave + m;
-            const f32x4_t vv = widen4(vc.raw(row, col));
-            const f32x4_t rr = *(const f32x4_t*)(rb + row * HD + col);
+        x.rr = *(const f32x4_t*)(rb + (16 * wave + m) * HD + col);
+        x.vv = widen4(vc.raw(16 * wave + m, col));
+    };
+    auto use = [&](const Operands& x) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) rdotv = fmaf(rr[r], vv[r], rdotv);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r) {
+            rdotv = fmaf(x.rr[r], x.vv[r], rdotv);
 #pragma unroll
             for (int n = 0; n < NN; ++n) {
-                gm = fmaf(bm[n][r], bg[n][r], gm);
+                gm = fmaf(x.m[n][r], x.g[n][r], gm);
 #pragma unroll
                 for (int it = 0; it < 4; ++it) {
-                    X[it][n] = mfma_f32(ao[it][r], bm[n][r], X[it][n]);
-                    Y[it][n] = mfma_f32(ar[it][r], bm[n][r], Y[it][n]);
-                    Z[it][n] = mfma_f32(au[it][r], bg[n][r], Z[it][n]);
+                    X[it][n] = mfma_f32(x.o[it][r], x.m[n][r], X[it][n]);
+                    Y[it][n] = mfma_f32(x.r[it][r], x.m[n][r], Y[it][n]);
+                    Z[it][n] = mfma_f32(x.u[it][r], x.g[n][r], Z[it][n]);
                 }
             }
+        }
+    };
+    Operands p0, p1;
+    load(p0, 0);
+#pragma unroll 1
+    for (int u = 0; u < HD / 16; u += 2) {
+        load(p1, u + 1);
+        use(p0);
+        if (u + 2 < HD / 16) load(p0, u + 2);
+        use(p1);
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) gm += __shfl_xor(gm, off);
@@ -861,6 +922,13 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
             }
         }
     __syncthreads();                               // dm, es, dg and the row sums are complete
+    if (wave == 0) {                               // the last row of the decays carries k_j.Z_j and <G, M> too
+        sky[lane] = red[0][1][lane] + red[1][1][lane] + red[2][1][lane] + red[3][1][lane];
+        float d = red[0][0][lane] + red[1][0][lane] + red[2][0][lane] + red[3][0][lane] - sb[lane] * sky[lane];
+        if (lane == DC - 1) d += fro[0] + fro[1] + fro[2] + fro[3];
+        else dg[lane][DC - 1] += red[0][2][lane] + red[1][2][lane] + red[2][2][lane] + red[3][2][lane];
+        sdg[lane] = d;
+    }
 #pragma unroll 1
     for (int jt = 0; jt < 4; ++jt) {
         f32x4_t ad[4], ae[4];
@@ -903,25 +971,44 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
                 dqc.put(i, col, X[it][n][r]);
                 dkc.put(i, col, Z[it][n][r]);
             }
-    __syncthreads();                               // dm is free
-    if (wave == 0) {
-        const float ky = red[0][1][lane] + red[1][1][lane] + red[2][1][lane] + red[3][1][lane];
-        const float qx = red[0][0][lane] + red[1][0][lane] + red[2][0][lane] + red[3][0][lane];
-        float w = qx - sb[lane] * ky;              // d(g_i)
-        if (lane == DC - 1) w += fro[0] + fro[1] + fro[2] + fro[3];
-        for (int t = 0; t < DC; ++t) {
-            dm[t][lane] = t <= lane ? gt[t][lane] * w : 0.f;
-            float d = t < lane ? dg[t][lane] : 0.f;
-            // the decays from every token to the chunk's end carry k_t.Z_t too
-            if (lane == DC - 1 && t < DC - 1) d += red[0][2][t] + red[1][2][t] + red[2][2][t] + red[3][2][t];
-            w = fmaf(sa[t], w, d);
+    // da_t: D[t][i] = sum_{j < t} g_{t-1,j} d(g_ij) + g_{t-1} d(g_i), weighted with g_it and summed over i >= t.  A wave takes
+    // the row tile `wave` of t.
+    __syncthreads();
+    {
+        const int t = 16 * wave + m;
+        float da[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            if (it < wave) continue;
+            const int i = 16 * it + m;
+            f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int jt = 0; jt < 4; ++jt) {
+                if (jt > wave) continue;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int j = 16 * jt + g4 + r;
+                    const float left_op = j < t ? gt[j][t - 1] : 0.f;
+                    d = mfma_f32(left_op, dg[j][i], d);
+                }
+            }
+            const float dgi = sdg[i];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int tt = 16 * wave + g4 + r;
+                const float before = tt > 0 ? sg[tt - 1] : 1.f;
+                if (i >= tt) da[r] = fmaf(gt[tt][i], fmaf(before, dgi, d[r]), da[r]);
+            }
         }
-        float da = 0.f;
-        for (int i = 0; i < DC; ++i) da += dm[lane][i];
-        if (lane < left) {
-            const int64_t at = (b * L + t0 + lane) * H + h;
-            DALPHA[at] = da;
-            DBETA[at] = sdb[0][lane] + sdb[1][lane] + sdb[2][lane] + sdb[3][lane] + srv[lane] - sg[lane] * ky;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int off = 1; off < 16; off <<= 1) da[r] += __shfl_xor(da[r], off);
+            const int tt = 16 * wave + g4 + r;
+            if (m == 0 && tt < left) DALPHA[(b * L + t0 + tt) * H + h] = da[r];
+        }
+        if (lane < 16 && t < left) {
+            DBETA[(b * L + t0 + t) * H + h] = sdb[0][t] + sdb[1][t] + sdb[2][t] + sdb[3][t] + srv[t] - sg[t] * sky[t];
         }
     }
 }
@@ -1035,35 +1122,37 @@ int launch_prep(const DeltaArgs& d, bf16_t* tf, bf16_t* tt, bf16_t* pf, float* g
     return VA_OK;
 }
 
-template <int HD, typename T, int W, bool OUT, bool SAVE>
+// The scans run four waves to a workgroup, one per SIMD.  Head dim 128 has eight groups of 16 columns: with one to a wave a
+// head takes two workgroups, which is shortest while there is a CU for each; from there on two to a wave halve the LDS reads
+// per product (the left operands serve both).
+constexpr int SCAN_W = 4;
+template <int HD> bool wide_scan(const DeltaArgs& d) { return HD == 128 && d.B * d.H > 128; }
+
+template <int HD, typename T, int CG, bool OUT, bool SAVE>
 int launch_scan(const DeltaArgs& d, const bf16_t* tf, const bf16_t* pf, const float* gam, const float* state_in, void* out,
                 float* state_out, float* us, float* ms, hipStream_t stream) {
-    constexpr int lds = ChunkRows<HD, T, W, OUT, parts<T>::MID, OUT ? parts<T>::OUT : 0>::LDS;
-    const auto fn = delta_scan_kernel<HD, T, W, OUT, SAVE>;
+    constexpr int lds = ChunkRows<HD, T, SCAN_W, OUT, parts<T>::MID, OUT ? parts<T>::OUT : 0>::LDS;
+    const auto fn = delta_scan_kernel<HD, T, SCAN_W, CG, OUT, SAVE>;
     VA_TRY(reserve_lds("va_gated_delta", (const void*)fn, lds));
-    hipLaunchKernelGGL(fn, dim3((unsigned)(d.B * d.H * (HD / 16 / W))), dim3(64 * W), lds, stream, (const T*)d.q, (const T*)d.k,
-                       (const T*)d.v, Rows{d.ldq}, Rows{d.ldk}, Rows{d.ldv}, d.beta, tf, pf, gam, state_in, (T*)out, state_out, us,
-                       ms, (int)d.L, (int)d.H, (int)d.chunks());
+    hipLaunchKernelGGL(fn, dim3((unsigned)(d.B * d.H * (HD / 16 / (SCAN_W * CG)))), dim3(64 * SCAN_W), lds, stream, (const T*)d.q,
+                       (const T*)d.k, (const T*)d.v, Rows{d.ldq}, Rows{d.ldk}, Rows{d.ldv}, d.beta, tf, pf, gam, state_in, (T*)out,
+                       state_out, us, ms, (int)d.L, (int)d.H, (int)d.chunks());
     VA_CHECK_LAUNCH("va_gated_delta (scan)");
     return VA_OK;
 }
 
-template <int HD, typename T, int W>
+template <int HD, typename T, int CG>
 int launch_rscan(const DeltaArgs& d, const void* d_out, const bf16_t* tt, const bf16_t* pt, const float* gam, const float* d_state,
                  void* dv, float* d_state_in, float* rs, float* gs, hipStream_t stream) {
-    constexpr int lds = ChunkRows<HD, T, W, true, parts<T>::MID, parts<T>::MID>::LDS;
-    const auto fn = delta_rscan_kernel<HD, T, W>;
+    constexpr int lds = ChunkRows<HD, T, SCAN_W, true, parts<T>::MID, parts<T>::MID>::LDS;
+    const auto fn = delta_rscan_kernel<HD, T, SCAN_W, CG>;
     VA_TRY(reserve_lds("va_gated_delta_bwd", (const void*)fn, lds));
-    hipLaunchKernelGGL(fn, dim3((unsigned)(d.B * d.H * (HD / 16 / W))), dim3(64 * W), lds, stream, (const T*)d.q, (const T*)d.k,
-                       Rows{d.ldq}, Rows{d.ldk}, (const T*)d_out, d.beta, tt, pt, gam, d_state, (T*)dv, d_state_in, rs, gs,
-                       (int)d.L, (int)d.H, (int)d.chunks());
+    hipLaunchKernelGGL(fn, dim3((unsigned)(d.B * d.H * (HD / 16 / (SCAN_W * CG)))), dim3(64 * SCAN_W), lds, stream, (const T*)d.q,
+                       (const T*)d.k, Rows{d.ldq}, Rows{d.ldk}, (const T*)d_out, d.beta, tt, pt, gam, d_state, (T*)dv, d_state_in, rs,
+                       gs, (int)d.L, (int)d.H, (int)d.chunks());
     VA_CHECK_LAUNCH("va_gated_delta_bwd (scan)");
     return VA_OK;
 }
-
-// Waves per workgroup of the scans: a wave's work does not depend on it, only how many waves share one copy of a chunk's
-// rows.  Few heads are spread over as many CUs as there are pairs of waves, many heads keep all columns together.
-int scan_waves(int64_t heads, int hd) { return heads * (hd / 16) >= 8 * 256 ? hd / 16 : 2; }
 
 // bytes of one chunk's share of a workspace
 constexpr int64_t OPERAND_BYTES = BLK * BFRAG * 2;
@@ -1078,9 +1167,8 @@ int delta_fwd(const DeltaArgs& d, const float* state_in, void* out, float* state
     bf16_t* pf = w.take<bf16_t>(n * BLK * BFRAG * parts<T>::OUT);
     float* gam = w.take<float>(n * 2 * DC);
     VA_TRY((launch_prep<HD, T, false>(d, tf, nullptr, pf, gam, stream)));
-    if (scan_waves(d.B * d.H, HD) == 2)
-        return launch_scan<HD, T, 2, true, false>(d, tf, pf, gam, state_in, out, state_out, nullptr, nullptr, stream);
-    return launch_scan<HD, T, HD / 16, true, false>(d, tf, pf, gam, state_in, out, state_out, nullptr, nullptr, stream);
+    if (wide_scan<HD>(d)) return launch_scan<HD, T, HD / 64, true, false>(d, tf, pf, gam, state_in, out, state_out, nullptr, nullptr, stream);
+    return launch_scan<HD, T, 1, true, false>(d, tf, pf, gam, state_in, out, state_out, nullptr, nullptr, stream);
 }
 
 template <int HD, typename T>
@@ -1092,14 +1180,14 @@ int delta_bwd(const DeltaArgs& d, const void* d_out, const float* d_state, const
     float *gam = w.take<float>(n * 2 * DC), *us = w.take<float>(n * DC * HD), *rs = w.take<float>(n * DC * HD);
     float *ms = w.take<float>(n * HD * HD), *gs = w.take<float>(n * HD * HD);
     VA_TRY((launch_prep<HD, T, true>(d, tf, tt, pt, gam, stream)));
-    if (scan_waves(d.B * d.H, HD) == 2) {
-        VA_TRY((launch_scan<HD, T, 2, false, true>(d, tf, nullptr, gam, state_in, nullptr, nullptr, us, ms, stream)));
-        VA_TRY((launch_rscan<HD, T, 2>(d, d_out, tt, pt, gam, d_state, dv, d_state_in, rs, gs, stream)));
+    if (wide_scan<HD>(d)) {
+        VA_TRY((launch_scan<HD, T, HD / 64, false, true>(d, tf, nullptr, gam, state_in, nullptr, nullptr, us, ms, stream)));
+        VA_TRY((launch_rscan<HD, T, HD / 64>(d, d_out, tt, pt, gam, d_state, dv, d_state_in, rs, gs, stream)));
     } else {
-        VA_TRY((launch_scan<HD, T, HD / 16, false, true>(d, tf, nullptr, gam, state_in, nullptr, nullptr, us, ms, stream)));
-        VA_TRY((launch_rscan<HD, T, HD / 16>(d, d_out, tt, pt, gam, d_state, dv, d_state_in, rs, gs, stream)));
+        VA_TRY((launch_scan<HD, T, 1, false, true>(d, tf, nullptr, gam, state_in, nullptr, nullptr, us, ms, stream)));
+        VA_TRY((launch_rscan<HD, T, 1>(d, d_out, tt, pt, gam, d_state, dv, d_state_in, rs, gs, stream)));
     }
-    constexpr int lds = (2 * DC * (HD + 4) + 4 * DC * SQ + 3 * DC + 4 * DC + 12 * DC + DC + 4) * 4;
+    constexpr int lds = (2 * DC * (HD + 4) + 4 * DC * SQ + 3 * DC + 4 * DC + 12 * DC + DC + 4 + 2 * DC) * 4;
     const auto fn = delta_grad_kernel<HD, T>;
     VA_TRY(reserve_lds("va_gated_delta_bwd", (const void*)fn, lds));
     hipLaunchKernelGGL(fn, dim3((unsigned)n), dim3(256), lds, stream, (const T*)d.q, (const T*)d.k, (const T*)d.v, Rows{d.ldq},
