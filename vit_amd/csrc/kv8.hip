@@ -125,6 +125,12 @@ __global__ __launch_bounds__(256) void kv8_advance_kernel(int32_t* __restrict__ 
 // ---- attention ------------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2v_t;
 
+// 16 bytes at `at` of a span that starts at a wave-uniform address; zeros behind its end
+VA_DEVINL u32x4_t span16(const void* base, int bytes, int at) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes, 0x00020000);
+    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+}
+
 // eight codes -> eight bf16 numbers, times the block's scale: exact
 VA_DEVINL u32x4_t widen8(uint32_t lo, uint32_t hi, float scale) {
     u32x4_t r;
@@ -167,8 +173,9 @@ VA_DEVINL void stream_lengths(const AttnArgs& a, const Cache& c, int b, int& len
     nb = nb < 0 ? 0 : nb > a.n ? a.n : nb;
 }
 
-// Softmax weights of one 64-key tile for 16 queries and the rescaled running state.  s[kt] = scores (times nothing yet) of
-// keys 16 kt + 4 g + r; pf[u] = the tile's P^T operand for keys 32 u ..+31.
+// Softmax weights of one 64-key tile for 16 queries and the rescaled running state.  s[kt] = raw scores of keys 16 kt + 4 g + r;
+// pf[u] = the tile's P^T operand for keys 32 u ..+31.  The running maximum is one of raw scores (the scale is positive), the
+// scale goes into the exponent's multiply-add.
 template <bool MASK>
 VA_DEVINL float tile_softmax(f32x4_t (&s)[4], int key0, int g4, int limit, float scale2, float& mx, float& sum, bf16x8_t (&pf)[2]) {
     float top = NEG_INF;
@@ -176,16 +183,14 @@ VA_DEVINL float tile_softmax(f32x4_t (&s)[4], int key0, int g4, int limit, float
     for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            float x = s[kt][r] * scale2;
-            if (MASK) x = key0 + 16 * kt + g4 + r < limit ? x : NEG_INF;
-            s[kt][r] = x;
-            top = fmaxf(top, x);
+            if (MASK) s[kt][r] = key0 + 16 * kt + g4 + r < limit ? s[kt][r] : NEG_INF;
+            top = fmaxf(top, s[kt][r]);
         }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     const float now = fmaxf(mx, top);
-    const float base = now == NEG_INF ? 0.f : now;         // nothing seen yet: every weight is exp2(-inf) = 0
-    const float fade = __builtin_amdgcn_exp2f(mx - base);
+    const float base = now == NEG_INF ? 0.f : now * scale2;     // nothing seen yet: every weight is exp2(-inf) = 0
+    const float fade = __builtin_amdgcn_exp2f(fmaf(mx, scale2, -base));
     mx = now;
     float add = 0.f;
     uint32_t pk[4][2];
@@ -193,13 +198,13 @@ VA_DEVINL float tile_softmax(f32x4_t (&s)[4], int key0, int g4, int limit, float
     for (int kt = 0; kt < 4; ++kt) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[kt][r] = __builtin_amdgcn_exp2f(s[kt][r] - base);
+            s[kt][r] = __builtin_amdgcn_exp2f(fmaf(s[kt][r], scale2, -base));
             add += s[kt][r];
         }
         pk[kt][0] = pack_bf16x2(s[kt][0], s[kt][1]);
         pk[kt][1] = pack_bf16x2(s[kt][2], s[kt][3]);
     }
-    sum = sum * fade + add;                                // this lane's share: its own keys
+    sum = fmaf(sum, fade, add);                                 // this lane's share: its own keys
 #pragma unroll
     for (int u = 0; u < 2; ++u) pf[u] = as_frag((u32x4_t){pk[2 * u][0], pk[2 * u][1], pk[2 * u + 1][0], pk[2 * u + 1][1]});
     return fade;
@@ -265,7 +270,7 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Cache c, AttnArgs a)
     constexpr int NP = HD / 16;              // 16-byte pieces of a 64-key tile per lane
     __shared__ __align__(16) char lds[4 * KB * VSTR];
     __shared__ float sml[4][2][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4, g4 = g * 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4, g4 = g * 4;
     const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     const int rows = a.n * a.G;
     int len, nb;
@@ -278,8 +283,7 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Cache c, AttnArgs a)
     most = __builtin_amdgcn_readfirstlane(most);            // the four lane groups hold the same queries
     least = __builtin_amdgcn_readfirstlane(least);
     const int tiles = (most + KB - 1) / KB, full = len / KB;         // tiles below `full` are in 8 bits, the next is the open one
-    const uint8_t* kb = c.k8 + bh * c.cap * HD + m * HD + g * (HD / 4);
-    const uint8_t* vb = c.v8 + bh * c.cap * HD;
+    const uint8_t *kb = c.k8 + bh * c.cap * HD, *vb = c.v8 + bh * c.cap * HD;
     const float *ksp = c.ks + bh * (c.cap / KB), *vsp = c.vs + bh * (c.cap / KB);
     char* vt = lds + wave * KB * VSTR;
     // queries: row m, the HD/4 elements that this lane group's key pieces hold
@@ -302,9 +306,9 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Cache c, AttnArgs a)
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-            for (int x = 0; x < NK; ++x) kr[kt][x] = *(const u32x4_t*)(kb + at + kt * 16 * HD + x * 16);
+            for (int x = 0; x < NK; ++x) kr[kt][x] = span16(kb + at, KB * HD, (kt * 16 + m) * HD + g * (HD / 4) + x * 16);
 #pragma unroll
-        for (int x = 0; x < NP; ++x) vr[x] = *(const u32x4_t*)(vb + at + (x * 64 + lane) * 16);
+        for (int x = 0; x < NP; ++x) vr[x] = span16(vb + at, KB * HD, (x * 64 + lane) * 16);
         kscale = ksp[t];
         vscale = vsp[t];
     };
@@ -329,7 +333,7 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Cache c, AttnArgs a)
             for (int x = 0; x < NP; ++x) {
                 const int idx = x * 64 + lane, row = idx / (HD / 16), col = (idx % (HD / 16)) * 16;
                 const u32x4_t lo = widen8(vr[x][0], vr[x][1], vscale), hi = widen8(vr[x][2], vr[x][3], vscale);
-                bad |= any_nonfinite(lo) || any_nonfinite(hi);
+                if (edge) bad |= any_nonfinite(lo) || any_nonfinite(hi);
                 *(u32x4_t*)(vt + row * VSTR + col * 2) = lo;
                 *(u32x4_t*)(vt + row * VSTR + col * 2 + 16) = hi;
             }
@@ -343,13 +347,12 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Cache c, AttnArgs a)
                 s[kt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int f = 0; f < HD / 32; ++f)
-                    s[kt] = mfma16(as_frag(*(const u32x4_t*)(ko + (16 * kt + m) * HD + g * (HD / 4) + 8 * f)), qf[f], s[kt]);
+                    s[kt] = mfma16(as_frag(span16(ko, left * HD * 2, ((16 * kt + m) * HD + g * (HD / 4) + 8 * f) * 2)), qf[f], s[kt]);
             }
 #pragma unroll
             for (int x = 0; x < 2 * NP; ++x) {
                 const int idx = x * 64 + lane, row = idx / (HD / 8), col = (idx % (HD / 8)) * 8;
-                u32x4_t v = {0u, 0u, 0u, 0u};            // behind the stream's end: nothing that was left there counts
-                if (row < left) v = *(const u32x4_t*)(vo + row * HD + col);
+                const u32x4_t v = span16(vo, left * HD * 2, idx * 16);      // zeros behind the stream's end, whatever lies there
                 bad |= any_nonfinite(v);
                 *(u32x4_t*)(vt + row * VSTR + col * 2) = v;
             }
@@ -380,7 +383,7 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Cache c, AttnArgs a)
         f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = sml[w][0][row] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(sml[w][0][row] - top);
+            const float f = sml[w][0][row] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((sml[w][0][row] - top) * a.scale2);
             total = fmaf(f, sml[w][1][row], total);
             if (f != 0.f) acc += f * *(const f32x4_t*)(so + (w * 16 + row) * OSTR + col);
         }
@@ -406,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
     constexpr int N = KB * HD / 16 / 256;    // 16-byte pieces of a tile per thread
     extern __shared__ __align__(16) char lds[];
     __shared__ int sbad[2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4, g4 = g * 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4, g4 = g * 4;
     const int rows = a.n * a.G, h = blockIdx.y, b = blockIdx.z;
     const int split = blockIdx.x % a.splits, row0 = (int)(blockIdx.x / a.splits) * 128 + wave * 32;
     int len, nb;
@@ -416,12 +419,12 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
     const float *ksp = c.ks + bh * (c.cap / KB), *vsp = c.vs + bh * (c.cap / KB);
     const int full = len / KB;
     // the workgroup's last visible key: limits do not fall with the row
-    const int last_row = min((int)(blockIdx.x / a.splits) * 128 + 127, rows - 1);
-    int most = 0;
-    {
-        const int q = min(last_row / a.G, nb - 1);
-        if (q >= 0) most = key_limit(a, q, len, nb);
-    }
+    const int first_row = (int)(blockIdx.x / a.splits) * 128, last_row = min(first_row + 127, rows - 1);
+    const int last_q = min(last_row / a.G, nb - 1);
+    const int most = last_q >= first_row / a.G ? key_limit(a, last_q, len, nb) : 0;
+    // keys that every row of the workgroup sees
+    const int all_see = last_row / a.G < nb ? key_limit(a, first_row / a.G, len, nb) : 0;
+    const bool idle = row0 >= rows;          // a wave without rows only helps to load
     const int tiles = (most + KB - 1) / KB;
     const int per = (tiles + a.splits - 1) / a.splits, t_begin = split * per, t_end = min(tiles, t_begin + per);
     bf16x8_t qf[2][HD / 32];
@@ -455,40 +458,45 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
         const int64_t at = (int64_t)t * KB * HD;
 #pragma unroll
         for (int p = 0; p < N; ++p) {
-            kr[p] = *(const u32x4_t*)(kb + at + (p * 256 + tid) * 16);
-            vr[p] = *(const u32x4_t*)(vb + at + (p * 256 + tid) * 16);
+            kr[p] = span16(kb + at, KB * HD, (p * 256 + tid) * 16);
+            vr[p] = span16(vb + at, KB * HD, (p * 256 + tid) * 16);
         }
         kscale = ksp[t];
         vscale = vsp[t];
     };
     auto place = [&](int t) {                // requested bytes (or the open block) into the tile's buffer
         if (t >= t_end) return;
-        char *kt_ = lds + (t & 1) * BUF, *vt_ = kt_ + KB * KSTR;
         bool bad = false;
+        const bool look = (t + 1) * KB > all_see;
+        // everything below is an immediate away from the thread's first piece; the compiler would keep each sum in a
+        // register over the loop (and spill it) if it could see that they do not change
+        int id = tid;
+        asm volatile("" : "+v"(id));
         if (t < full) {
+            constexpr int C = HD / 16, ROWS = 256 / C;      // pieces of a row, rows of a pass
+            char* kt_ = lds + (t & 1) * BUF + (id / C) * KSTR + (id % C) * 32;
+            char* vt_ = lds + (t & 1) * BUF + KB * KSTR + (id / C) * VSTR + (id % C) * 32;
 #pragma unroll
             for (int p = 0; p < N; ++p) {
-                const int idx = p * 256 + tid, row = idx / (HD / 16), col = (idx % (HD / 16)) * 32;
-                *(u32x4_t*)(kt_ + row * KSTR + col) = widen8(kr[p][0], kr[p][1], kscale);
-                *(u32x4_t*)(kt_ + row * KSTR + col + 16) = widen8(kr[p][2], kr[p][3], kscale);
+                *(u32x4_t*)(kt_ + p * ROWS * KSTR) = widen8(kr[p][0], kr[p][1], kscale);
+                *(u32x4_t*)(kt_ + p * ROWS * KSTR + 16) = widen8(kr[p][2], kr[p][3], kscale);
                 const u32x4_t lo = widen8(vr[p][0], vr[p][1], vscale), hi = widen8(vr[p][2], vr[p][3], vscale);
-                bad |= any_nonfinite(lo) || any_nonfinite(hi);
-                *(u32x4_t*)(vt_ + row * VSTR + col) = lo;
-                *(u32x4_t*)(vt_ + row * VSTR + col + 16) = hi;
+                if (look) bad |= any_nonfinite(lo) || any_nonfinite(hi);
+                *(u32x4_t*)(vt_ + p * ROWS * VSTR) = lo;
+                *(u32x4_t*)(vt_ + p * ROWS * VSTR + 16) = hi;
             }
         } else {
+            constexpr int C = HD / 8, ROWS = 256 / C;
             const int left = len - t * KB;
+            char* kt_ = lds + (t & 1) * BUF + (id / C) * KSTR + (id % C) * 16;
+            char* vt_ = lds + (t & 1) * BUF + KB * KSTR + (id / C) * VSTR + (id % C) * 16;
 #pragma unroll
             for (int p = 0; p < 2 * N; ++p) {
-                const int idx = p * 256 + tid, row = idx / (HD / 8), col = (idx % (HD / 8)) * 8;
-                u32x4_t k = {0u, 0u, 0u, 0u}, v = k;
-                if (row < left) {
-                    k = *(const u32x4_t*)(c.ko + (bh * KB + row) * HD + col);
-                    v = *(const u32x4_t*)(c.vo + (bh * KB + row) * HD + col);
-                }
+                const u32x4_t k = span16(c.ko + bh * KB * HD, left * HD * 2, (p * 256 + id) * 16);
+                const u32x4_t v = span16(c.vo + bh * KB * HD, left * HD * 2, (p * 256 + id) * 16);
                 bad |= any_nonfinite(v);
-                *(u32x4_t*)(kt_ + row * KSTR + col * 2) = k;
-                *(u32x4_t*)(vt_ + row * VSTR + col * 2) = v;
+                *(u32x4_t*)(kt_ + p * ROWS * KSTR) = k;
+                *(u32x4_t*)(vt_ + p * ROWS * VSTR) = v;
             }
         }
         if (bad) sbad[t & 1] = 1;            // every writer writes the same
@@ -503,6 +511,9 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
         const bool flagged = sbad[t & 1] != 0;
         place(t + 1);
         request(t + 2);
+        if (idle) continue;
+        int ln = lane;                       // as in place(): addresses are formed anew instead of kept and spilled
+        asm volatile("" : "+v"(ln));
         const char *kt_ = lds + (t & 1) * BUF, *vt_ = kt_ + KB * KSTR;
         f32x4_t s[2][4];
 #pragma unroll
@@ -510,7 +521,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
             s[0][kt] = s[1][kt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int f = 0; f < HD / 32; ++f) {
-                const bf16x8_t kf = as_frag(*(const u32x4_t*)(kt_ + (16 * kt + m) * KSTR + (32 * f + 8 * g) * 2));
+                const bf16x8_t kf = as_frag(*(const u32x4_t*)(kt_ + (ln & 15) * KSTR + (ln >> 4) * 16 + 16 * kt * KSTR + 64 * f));
                 s[0][kt] = mfma16(kf, qf[0][f], s[0][kt]);
                 s[1][kt] = mfma16(kf, qf[1][f], s[1][kt]);
             }
@@ -525,14 +536,14 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
             for (int ht = 0; ht < HD / 16; ++ht) o[ct][ht] *= fade;
         }
         if (edge && flagged) {
-            tile_pv<HD>(vt_, VSTR, pf[0], o[0], lane, true, limit[0] - t * KB);
-            tile_pv<HD>(vt_, VSTR, pf[1], o[1], lane, true, limit[1] - t * KB);
+            tile_pv<HD>(vt_, VSTR, pf[0], o[0], ln, true, limit[0] - t * KB);
+            tile_pv<HD>(vt_, VSTR, pf[1], o[1], ln, true, limit[1] - t * KB);
         } else {
 #pragma unroll
             for (int ht = 0; ht < HD / 16; ++ht)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const bf16x8_t vf = v_frag(vt_, VSTR, ht, u, lane);
+                    const bf16x8_t vf = v_frag(vt_, VSTR, ht, u, ln);
                     o[0][ht] = mfma16(vf, pf[0][u], o[0][ht]);
                     o[1][ht] = mfma16(vf, pf[1][u], o[1][ht]);
                 }
@@ -575,7 +586,7 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a) {
     for (int s = 0; s < a.splits; ++s) {
         const float mx = a.part_ml[2 * (s * all + idx)];
         if (mx == NEG_INF) continue;
-        const float f = __builtin_amdgcn_exp2f(mx - top);
+        const float f = __builtin_amdgcn_exp2f((mx - top) * a.scale2);
         total = fmaf(f, a.part_ml[2 * (s * all + idx) + 1], total);
         acc += f * *(const f32x4_t*)(a.part_o + (s * all + idx) * HD + col);
     }
@@ -592,7 +603,8 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a) {
 // never a piece below four tiles per wave (few rows) or per workgroup (many rows).  `max_len` only steers this.
 int kv8_splits(int64_t B, int64_t H, int64_t rows, int64_t max_len) {
     const int64_t groups = B * H * (rows <= 16 ? 1 : (rows + 127) / 128), tiles = (max_len + KB - 1) / KB;
-    int64_t s = (2 * 256 + groups - 1) / groups;
+    const int64_t want = rows <= 16 ? 2 * 256 : 256;
+    int64_t s = (want + groups - 1) / groups;
     const int64_t most = rows <= 16 ? (tiles + 15) / 16 : (tiles + 3) / 4;
     s = s < most ? s : most;
     return (int)(s < 1 ? 1 : s > 128 ? 128 : s);
@@ -677,6 +689,7 @@ extern "C" int va_kv8_attn(const void* q, int64_t ldq, int64_t bsq, const int32_
                  "va_kv8_attn: the token stride of q must be at least its heads' width, and the strides multiples of 8");
     VA_CHECK_ARG(tokens_per_timestep >= 0 && tokens_per_timestep < (1ll << 30), "va_kv8_attn: tokens per timestep out of range");
     VA_CHECK_ARG(max_len >= 0 && max_len <= cap, "va_kv8_attn: max_len out of range");
+    VA_CHECK_ARG(scale > 0.f && scale < 1e30f, "va_kv8_attn: the scale must be positive");
     const int splits = kv8_splits(B, H, n * group, max_len);
     VA_CHECK_ARG(splits == 1 || workspace, "va_kv8_attn: null workspace");
     const Cache c = {(const uint8_t*)k8, (const uint8_t*)v8, k_scale, v_scale, (const bf16_t*)k_open, (const bf16_t*)v_open, lengths, cap};

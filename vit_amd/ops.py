@@ -429,9 +429,9 @@ class KVCache8:
                                       ("v_scale", v_scale, F32, (B, H, cap // KV8_BLOCK)),
                                       ("k_open", k_open, BF16, (B, H, KV8_BLOCK, hd)), ("v_open", v_open, BF16, (B, H, KV8_BLOCK, hd)),
                                       ("lengths", lengths, torch.int32, (B,))):
-            _need(t, dtype, name)
             if t.shape != shape or not t.is_contiguous():
                 raise ValueError(f"KVCache8: {name} must be contiguous {shape}")
+            _need(t, dtype, name)
         if max_len is not None and not 0 <= max_len <= cap:
             raise ValueError("KVCache8: max_len must lie between 0 and the capacity")
         self.k8, self.v8, self.k_scale, self.v_scale = k8, v8, k_scale, v_scale
@@ -449,6 +449,12 @@ class KVCache8:
         opened = [new(BF16, KV8_BLOCK, head_dim) for _ in range(2)]
         return cls(*codes, *scales, *opened, torch.zeros(batch, dtype=torch.int32, device=device), max_len=0)
 
+    def pointers(self):
+        """Addresses of the seven tensors, in the order of the C entry points."""
+        if self.k8.get_device() != _current_device():
+            raise _lib.VitAmdError(f"KVCache8: the cache is on {self.k8.device} but the current device is cuda:{_current_device()}")
+        return tuple(t.data_ptr() for t in (self.k8, self.v8, self.k_scale, self.v_scale, self.k_open, self.v_open, self.lengths))
+
     def reset(self) -> None:
         """Forget all tokens."""
         self.lengths.zero_()
@@ -458,18 +464,19 @@ class KVCache8:
 def _token_strides(t: torch.Tensor, name: str, shape) -> Tuple[int, int]:
     """(elements between tokens, between streams) of bf16 [B, n, heads, hd] with the heads of a token side by side."""
     _need(t, BF16, name)
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.stride(3) != 1 or (t.shape[2] > 1 and t.stride(2) != t.shape[3]):
+    B, n, H, hd = shape
+    stream, token, head, one = t.stride()
+    if one != 1 or (H > 1 and head != hd):
         raise ValueError(f"{name}: the heads of a token must lie side by side")
-    return (t.stride(1) if t.shape[1] > 1 else t.shape[2] * t.shape[3]), (t.stride(0) if t.shape[0] > 1 else 0)
+    return (token if n > 1 else H * hd), (stream if B > 1 else 0)
 
 
-def _new_tokens(new: Optional[torch.Tensor], B: int):
-    if new is not None:
-        _need(new, torch.int32, "new")
-        if tuple(new.shape) != (B,) or not new.is_contiguous():
-            raise ValueError("new must be a contiguous int32 [B] tensor")
+def _new_tokens(new: torch.Tensor, B: int):
+    _need(new, torch.int32, "new")
+    if tuple(new.shape) != (B,) or not new.is_contiguous():
+        raise ValueError("new must be a contiguous int32 [B] tensor")
 
 
 def kv8_append_(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, new: Optional[torch.Tensor] = None) -> KVCache8:
@@ -482,11 +489,11 @@ def kv8_append_(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, new: Optional
     n = k.shape[1]
     ldk, bsk = _token_strides(k, "k", (B, n, H, hd))
     ldv, bsv = _token_strides(v, "v", (B, n, H, hd))
-    _new_tokens(new, B)
+    if new is not None:
+        _new_tokens(new, B)
     if cache.max_len + n > cache.capacity:
         raise ValueError(f"kv8_append_: {n} tokens behind up to {cache.max_len} pass the capacity of {cache.capacity}")
-    check(_lib.load().va_kv8_append(_p(k), _p(v), ldk, ldv, bsk, bsv, _p(new), n, _p(cache.k8), _p(cache.v8), _p(cache.k_scale),
-                                    _p(cache.v_scale), _p(cache.k_open), _p(cache.v_open), _p(cache.lengths), B, H, hd,
+    check(_lib.load().va_kv8_append(k.data_ptr(), v.data_ptr(), ldk, ldv, bsk, bsv, _p(new), n, *cache.pointers(), B, H, hd,
                                     cache.capacity, _stream()), "va_kv8_append")
     cache.max_len += n
     return cache
@@ -503,15 +510,15 @@ def kv8_attn(q: torch.Tensor, cache: KVCache8, new: Optional[torch.Tensor] = Non
         raise ValueError("kv8_attn: q must be [B, n, heads, hd] with heads a multiple of the cache's")
     n, Hq = q.shape[1], q.shape[2]
     ldq, bsq = _token_strides(q, "q", (B, n, Hq, hd))
-    _new_tokens(new, B)
+    if new is not None:
+        _new_tokens(new, B)
     if tokens_per_timestep < 0:
         raise ValueError("kv8_attn: tokens_per_timestep must not be negative")
     lib = _lib.load()
     out = torch.empty(B, n, Hq, hd, dtype=BF16, device=q.device)
     floats = lib.va_kv8_attn_workspace_floats(B, n, H, Hq // H, hd, cache.max_len)
     ws = torch.empty(floats, dtype=F32, device=q.device) if floats else None
-    check(lib.va_kv8_attn(_p(q), ldq, bsq, _p(new), _p(cache.k8), _p(cache.v8), _p(cache.k_scale), _p(cache.v_scale),
-                          _p(cache.k_open), _p(cache.v_open), _p(cache.lengths), _p(out), _p(ws), B, n, H, Hq // H, hd,
+    check(lib.va_kv8_attn(q.data_ptr(), ldq, bsq, _p(new), *cache.pointers(), out.data_ptr(), _p(ws), B, n, H, Hq // H, hd,
                           cache.capacity, cache.max_len, tokens_per_timestep, hd ** -0.5 if scale is None else float(scale),
                           _stream()), "va_kv8_attn")
     return out
