@@ -34,6 +34,15 @@ def block_supported(blk, x: torch.Tensor) -> bool:
             and blk.spatial_attn._qkv_same_embed_dim)
 
 
+def delta_rule(q, k, v, alpha, beta, state):
+    """The memory layer's recurrence without a graph: token by token below 64 tokens (512 heads x 32 tokens of head dim 128:
+    40 against 58 us; one stream of 8 heads: 22 against 22), chunks of 64 from there on (512 x 64: 61 against 65 us, 512 x 2064:
+    1.24 against 1.67 ms; 8 x 258: 47 against 151 us).  The two add the same f32 products in another order."""
+    if q.shape[1] < 64:
+        return ops.gated_delta_seq(q, k, v, alpha, beta, state)
+    return ops.gated_delta_fwd(q, k, v, alpha, beta, state)
+
+
 def block_forward(blk, x: torch.Tensor, tokens_per_timestep: int, state: Optional[torch.Tensor],
                   wc: WeightCache) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """x f32 [B, L, D] on the device; tokens_per_timestep 0 = no mask.  Returns (x_out [B,L,D], new state)."""
@@ -81,8 +90,8 @@ def block_forward(blk, x: torch.Tensor, tokens_per_timestep: int, state: Optiona
         k = ops.dwconv1d_causal_silu_bf16(col(1), B, L, t.k_conv1d.weight.detach(), t.k_conv1d.bias.detach(), True)
         v = ops.dwconv1d_causal_silu_bf16(col(2), B, L, conv_w[:inner], conv_b[:inner], False)
         v_gate = ops.dwconv1d_causal_silu_bf16(col(3), B, L, conv_w[inner:], conv_b[inner:], False)
-        out, new_state = ops.gated_delta_seq(q.view(B, L, Hd, Dh), k.view(B, L, Hd, Dh), v.view(B, L, Hd, Dh), alpha, beta,
-                                             None if state is None else state.detach().contiguous())
+        out, new_state = delta_rule(q.view(B, L, Hd, Dh), k.view(B, L, Hd, Dh), v.view(B, L, Hd, Dh), alpha, beta,
+                                    None if state is None else state.detach().contiguous())
         del q, k, v
         on = new(inner, BF16)
         ops.gate_layernorm_fwd(out.view(M, inner), v_gate.view(M, inner), col(4), t.o_norm.weight.detach(),

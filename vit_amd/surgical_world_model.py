@@ -424,8 +424,9 @@ def _note_torch_path(x: torch.Tensor, who: str) -> None:
 
 class GatedDeltaLayer(nn.Module):
     """Gated delta-rule memory layer (swm:431-555).  What is computed is the sequential recurrence: the form inference uses
-    and the one the reference's other ("parallel") path fails to reproduce.  Without a graph it runs token by token in one
-    kernel; with one (f32 on the device, head dim 64 or 128) chunk by chunk, differentiable in every input and the state."""
+    and the one the reference's other ("parallel") path fails to reproduce.  On the device (f32, head dim 64 or 128) short
+    sequences without a graph run token by token in one kernel, the others chunk by chunk, differentiable in every input and
+    the state."""
 
     def __init__(self, hidden_size, num_heads=4, head_dim=128, chunk_size=64):
         super().__init__()
@@ -473,9 +474,9 @@ class GatedDeltaLayer(nn.Module):
             k = ops.dwconv1d_causal_silu(self.k_proj(x), self.k_conv1d.weight, self.k_conv1d.bias, True)
             v = ops.dwconv1d_causal_silu(self.v_proj(x), self.v_conv1d.weight, self.v_conv1d.bias, False)
             v, v_gate = v.chunk(2, dim=-1)
-            out, new_state = ops.gated_delta_seq(q.view(B, L, H, Dh), k.view(B, L, H, Dh),
-                                                 v.contiguous().view(B, L, H, Dh), alpha.contiguous(), beta.contiguous(),
-                                                 None if state is None else state.contiguous())
+            out, new_state = predictor_engine.delta_rule(q.view(B, L, H, Dh), k.view(B, L, H, Dh),
+                                                         v.contiguous().view(B, L, H, Dh), alpha.contiguous(),
+                                                         beta.contiguous(), None if state is None else state.contiguous())
         else:
             if Dh in (64, 128):
                 _note_torch_path(x, "GatedDeltaLayer.forward")
