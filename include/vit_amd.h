@@ -313,19 +313,22 @@ int va_gated_delta_seq(const float* q, const float* k, const float* v, const flo
  * bf16 (is_bf16; 8-byte alignment is enough then); alpha, beta: contiguous f32 [B,L,H]; states f32 [B,H,hd,hd] (rows = value
  * index); out / gradients of q, k, v: contiguous [B,L,H,hd] of the inputs' type.  hd 64 or 128.  Products and states are
  * f32 whatever the type.  A non-finite token spreads over the 64-token chunk it lies in, earlier tokens included.
- *   fwd:  state_in NULL = zeros.  workspace: va_gated_delta_fwd_workspace_floats f32 values.
+ *   fwd:  state_in NULL = zeros.  workspace: va_gated_delta_fwd_workspace_floats f32 values.  kept: NULL, or
+ *         va_gated_delta_kept_floats f32 values that receive what the gradient needs besides the inputs.
  *   bwd:  d_out, and d_state (of the final state; NULL = zeros) -> dq, dk, dv, dalpha, dbeta [, d_state_in unless NULL];
- *         nothing is kept from the forward.  workspace: va_gated_delta_bwd_workspace_floats f32 values.
+ *         kept: the forward's for the same inputs, or NULL (then computed again).  workspace:
+ *         va_gated_delta_bwd_workspace_floats(.., have_kept) f32 values.
  *   step: q, k, v [B, ld*], alpha, beta [B,H]; `state` is updated in place; out [B,H,hd]. */
 int64_t va_gated_delta_fwd_workspace_floats(int64_t B, int64_t L, int64_t H, int64_t hd);
-int64_t va_gated_delta_bwd_workspace_floats(int64_t B, int64_t L, int64_t H, int64_t hd);
+int64_t va_gated_delta_kept_floats(int64_t B, int64_t L, int64_t H, int64_t hd);
+int64_t va_gated_delta_bwd_workspace_floats(int64_t B, int64_t L, int64_t H, int64_t hd, int have_kept);
 int va_gated_delta_fwd(const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv, int is_bf16,
                        const float* alpha, const float* beta, const float* state_in, void* out, float* state_out,
-                       float* workspace, int64_t B, int64_t L, int64_t H, int64_t hd, va_stream_t stream);
+                       float* workspace, float* kept, int64_t B, int64_t L, int64_t H, int64_t hd, va_stream_t stream);
 int va_gated_delta_bwd(const void* d_out, const float* d_state, const void* q, const void* k, const void* v, int64_t ldq,
                        int64_t ldk, int64_t ldv, int is_bf16, const float* alpha, const float* beta, const float* state_in,
                        void* dq, void* dk, void* dv, float* dalpha, float* dbeta, float* d_state_in, float* workspace,
-                       int64_t B, int64_t L, int64_t H, int64_t hd, va_stream_t stream);
+                       const float* kept, int64_t B, int64_t L, int64_t H, int64_t hd, va_stream_t stream);
 int va_gated_delta_step(const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv, int is_bf16,
                         const float* alpha, const float* beta, float* state, void* out, int64_t B, int64_t H, int64_t hd,
                         va_stream_t stream);

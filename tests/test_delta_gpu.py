@@ -270,3 +270,18 @@ def test_row_strides():
     for bad in (x[:, :4], x[:, ::2], x.transpose(0, 1), x.transpose(1, 2), x[..., ::2]):
         with pytest.raises(ValueError):
             _heads_ld(bad, "x")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,H,hd", [(2, 131, 2, 128), (1, 64, 3, 64), (33, 70, 4, 128)])
+def test_what_the_forward_keeps_equals_what_the_gradient_computes_again(B, L, H, hd, dtype):
+    from vit_amd import ops
+    args = gpu_args(inputs(B, L, H, hd, dtype, True, seed="dk"))
+    out, s, kept = ops.gated_delta_fwd(*args, keep=True)
+    one, s1 = ops.gated_delta_fwd(*args)
+    assert torch.equal(out, one) and torch.equal(s, s1)
+    for x, y in zip(ops.gated_delta_bwd(out, s, *args, kept=kept), ops.gated_delta_bwd(out, s, *args)):
+        assert torch.equal(x, y)
+    with pytest.raises(ValueError):
+        ops.gated_delta_bwd(out, s, *args, kept=kept[1:])

@@ -68,9 +68,10 @@ SIGNATURES = {
     "va_multi_adamw": (ci, [vp, vp, i64, cf, cf, cf, cf, cf, vp, cf, vp]),
     "va_gated_delta_seq": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp]),
     "va_gated_delta_fwd_workspace_floats": (i64, [i64, i64, i64, i64]),
-    "va_gated_delta_bwd_workspace_floats": (i64, [i64, i64, i64, i64]),
-    "va_gated_delta_fwd": (ci, [vp, vp, vp, i64, i64, i64, ci, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp]),
-    "va_gated_delta_bwd": (ci, [vp, vp, vp, vp, vp, i64, i64, i64, ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64,
+    "va_gated_delta_kept_floats": (i64, [i64, i64, i64, i64]),
+    "va_gated_delta_bwd_workspace_floats": (i64, [i64, i64, i64, i64, ci]),
+    "va_gated_delta_fwd": (ci, [vp, vp, vp, i64, i64, i64, ci, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp]),
+    "va_gated_delta_bwd": (ci, [vp, vp, vp, vp, vp, i64, i64, i64, ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64,
                                 i64, vp]),
     "va_gated_delta_step": (ci, [vp, vp, vp, i64, i64, i64, ci, vp, vp, vp, vp, i64, i64, i64, vp]),
     "va_kv8_append": (ci, [vp, vp, i64, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp]),

@@ -18,8 +18,8 @@
 //     db_i = sum_j dA_ij g_ij k_i.k_j + R_i.v_i - g_i k_i.Y_i
 //     da_t = sum_{i >= t} g_it w_t[i],  w_{t+1}[i] = a_t w_t[i] + d(g_it),  w_1[i] = d(g_i)
 // (the last line needs no division by a decay, so decays of zero are ordinary numbers; the decays themselves are running
-// products, never differences of logarithms).  delta_scan_kernel runs once more for U and the chunks' states, then
-// delta_rscan_kernel backwards, then delta_grad_kernel per chunk.
+// products, never differences of logarithms).  delta_rscan_kernel walks backwards, then delta_grad_kernel takes the chunks in
+// parallel, both from the forward's T^T, P^T, U and chunk states (kept by it, or formed again by its two kernels).
 //
 // Numbers on the matrix pipe.  The bf16 instruction (16x16x32) does sixteen times the products of the f32 one (16x16x4) per
 // cycle, so the scans split every f32 operand into three bf16 numbers, x = x0 + x1 + x2 with |x1| <= 2^-8 |x| and
@@ -189,15 +189,15 @@ VA_DEVINL void rows_to_lds(const ChunkOf<T>& src, float (*dst)[HD + 4], int tid)
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// One workgroup of four waves per chunk.  K K^T tiles are formed transposed, D[j][i] = k_j.k_i, so that a lane holds row i and
-// four consecutive j; the wave with row tile w of K K^T (w + 1 tiles) takes row tile 3 - w of Q K^T, five tiles to each.  GRAD:
-// T, T^T and P^T for the gradient's scans (then by column tiles, P^T's rows: 4 - w tiles), otherwise T and P.
-template <int HD, typename T, bool GRAD>
+// One workgroup of four waves per chunk.  K K^T and Q K^T tiles are formed transposed, D[j][i] = k_j.x_i, so that a lane holds
+// row i and four consecutive j; the wave with row tile w of K K^T (w + 1 tiles) takes row tile 3 - w of Q K^T, five tiles to
+// each.  Writes T and P; TRAIN: T^T and P^T as well, for the gradient's scan (P^T's tiles are formed the other way round).
+template <int HD, typename T, bool TRAIN>
 __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q, const T* __restrict__ K, Rows rq, Rows rk,
                                                          const float* __restrict__ ALPHA, const float* __restrict__ BETA,
-                                                         bf16_t* __restrict__ TF, bf16_t* __restrict__ TT, bf16_t* __restrict__ PF,
-                                                         float* __restrict__ GAM, int L, int H, int NC) {
-    constexpr int NM = parts<T>::MID, NP = GRAD ? parts<T>::MID : parts<T>::OUT;
+                                                         bf16_t* __restrict__ TF, bf16_t* __restrict__ PF, bf16_t* __restrict__ TT,
+                                                         bf16_t* __restrict__ PT, float* __restrict__ GAM, int L, int H, int NC) {
+    constexpr int NM = parts<T>::MID, NP = parts<T>::OUT;
     constexpr int KBYTES = DC * (HD + 4) * 4, ABYTES = DC * SQ * 4 + DC * 20 * 4;
     __shared__ __align__(16) char lds[(KBYTES > ABYTES ? KBYTES : ABYTES)];
     __shared__ float gt[DC][SQ];
@@ -218,29 +218,26 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q
     if (wave == 0) chunk_decays(mine, gt, lane);
     if (wave == 1) GAM[ci * 2 * DC + lane] = chunk_prefix(mine, lane);
     __syncthreads();
-    const int qt = GRAD ? wave : 3 - wave;        // this wave's rows of Q (GRAD: its rows of P^T)
-    f32x4_t kk[4], qk[4];                         // kk[jt]: rows `wave`; qk[jt]: rows qt (GRAD: qk[it], P^T's columns)
+    f32x4_t kk[4], qk[4], pt[4];                  // kk[jt]: rows `wave`; qk[jt]: rows 3 - wave; pt[it]: P^T's rows `wave`
 #pragma unroll
-    for (int x = 0; x < 4; ++x) kk[x] = qk[x] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    for (int x = 0; x < 4; ++x) kk[x] = qk[x] = pt[x] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     // one copy of the code per wave: which tiles it forms is then known to the compiler
     auto tiles = [&](auto wv) {
-        constexpr int WV = decltype(wv)::value, QT = GRAD ? WV : 3 - WV;
+        constexpr int WV = decltype(wv)::value, QT = 3 - WV;
 #pragma unroll
         for (int u = 0; u < HD / 16; ++u) {
             const int col = 16 * u + g4;
-            const f32x4_t mk = *(const f32x4_t*)&ks[16 * WV + m][col];
-            f32x4_t mq = mk;                      // GRAD: the rows of P^T are keys, the wave's own
-            if (!GRAD) mq = widen4(qc.raw(16 * QT + m, col));
+            const f32x4_t mk = *(const f32x4_t*)&ks[16 * WV + m][col], mq = widen4(qc.raw(16 * QT + m, col));
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 f32x4_t kx = {0.f, 0.f, 0.f, 0.f}, qx = kx;
-                if (x <= WV || (!GRAD && x <= QT)) kx = *(const f32x4_t*)&ks[16 * x + m][col];
-                if (GRAD && x >= WV) qx = widen4(qc.raw(16 * x + m, col));
+                if (x <= WV || x <= QT) kx = *(const f32x4_t*)&ks[16 * x + m][col];
+                if (TRAIN && x >= WV) qx = widen4(qc.raw(16 * x + m, col));
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     if (x <= WV) kk[x] = mfma_f32(kx[r], mk[r], kk[x]);
-                    if (!GRAD && x <= QT) qk[x] = mfma_f32(kx[r], mq[r], qk[x]);
-                    if (GRAD && x >= WV) qk[x] = mfma_f32(qx[r], mq[r], qk[x]);
+                    if (x <= QT) qk[x] = mfma_f32(kx[r], mq[r], qk[x]);
+                    if (TRAIN && x >= WV) pt[x] = mfma_f32(qx[r], mk[r], pt[x]);
                 }
             }
         }
@@ -252,7 +249,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q
     __syncthreads();                              // K has been read
     if (wave == 2) GAM[ci * 2 * DC + DC + lane] = gt[lane][DC - 1];
     {
-        const int i = 16 * wave + m;
+        const int i = 16 * wave + m, qt = 3 - wave;
         const float bi = sb[i];
 #pragma unroll
         for (int jt = 0; jt < 4; ++jt) {
@@ -269,16 +266,24 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q
         for (int x = 0; x < 4; ++x)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int ii = GRAD ? 16 * x + g4 + r : 16 * qt + m, j = GRAD ? 16 * wave + m : 16 * x + g4 + r;
-                qk[x][r] = ii >= j ? qk[x][r] * gt[j][ii] : 0.f;
+                const int pi = 16 * qt + m, pj = 16 * x + g4 + r;           // P
+                qk[x][r] = pi >= pj ? qk[x][r] * gt[pj][pi] : 0.f;
+                const int ti = 16 * x + g4 + r;                              // P^T, row i of this wave
+                if (TRAIN) pt[x][r] = ti >= i ? pt[x][r] * gt[i][ti] : 0.f;
             }
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-            if (GRAD ? 2 * u + 1 >= wave : 2 * u <= qt) {
+        for (int u = 0; u < 2; ++u) {
+            if (2 * u <= qt) {
                 bf16x8_t f[NP];
                 split(qk[2 * u], qk[2 * u + 1], f);
-                store_block(PF + ci * BLK * NP * BFRAG, GRAD ? up_block(wave, u) : low_block(qt, u), lane, f);
+                store_block(PF + ci * BLK * NP * BFRAG, low_block(qt, u), lane, f);
             }
+            if (TRAIN && 2 * u + 1 >= wave) {
+                bf16x8_t f[NM];
+                split(pt[2 * u], pt[2 * u + 1], f);
+                store_block(PT + ci * BLK * NM * BFRAG, up_block(wave, u), lane, f);
+            }
+        }
     }
     __syncthreads();
     // inverse of a diagonal block by forward substitution, lane = column
@@ -332,7 +337,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q
     for (int it = 0; it < 4; ++it)
 #pragma unroll
         for (int r = 0; r < 4; ++r) am[16 * it + g4 + r][16 * wave + m] = xb[it][r];     // zeros above the diagonal too
-    if (GRAD) {
+    if (TRAIN) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
             if (2 * u + 1 >= wave) {
@@ -411,19 +416,23 @@ VA_DEVINL void to_lds(const void* src, char* dst, int wave, int lane) {
     }
 }
 
-// What the two scans share: the next chunk's rows of K (and Q) on their way from memory to LDS.  LDS of a workgroup: K, Q, the
-// chunk's two 64x64 operands (NA and NB parts), b, g, g_C.
-template <int HD, typename T, int W, bool TWO, int NA, int NB>
+// What the two scans share: what the next chunk needs, on its way from memory to LDS: rows of K (and Q), the two 64x64
+// operands (NA and NB parts), b, g, g_C.  AHEAD: the operands wait in registers like the rows; without (two column groups
+// leave no registers) they are loaded straight to LDS while the chunk's products with the state are formed.
+template <int HD, typename T, int W, bool TWO, int NA, int NB, bool AHEAD>
 struct ChunkRows {
     typedef typename ChunkOf<T>::raw4 raw4;
     static constexpr int N = DC * HD / 4 / (64 * W), IN = parts<T>::IN, MATRIX = IN * DC * HD * 2;
-    static constexpr int A_BYTES = BLK * NA * BFRAG * 2, B_BYTES = BLK * NB * BFRAG * 2;
+    static constexpr int A_BYTES = BLK * NA * BFRAG * 2, B_BYTES = BLK * NB * BFRAG * 2, KBS = (A_BYTES + B_BYTES) / 1024;
     static constexpr int A_AT = (TWO ? 2 : 1) * MATRIX, B_AT = A_AT + A_BYTES, F_AT = B_AT + B_BYTES, LDS = F_AT + 3 * DC * 4;
+    static constexpr int NX = AHEAD ? (KBS + W - 1) / W : 1;
     const T *k, *q;                               // row 0 of this head
     int64_t ldk, ldq;
+    const bf16_t *a, *b;                          // operands of this head's chunk 0
     const float *beta, *gam;
-    int L, H, tid;
+    int L, H, tid, wave;
     raw4 kn[N], qn[TWO ? N : 1];
+    u32x4_t xn[NX];
     float bn, gn, en;
     VA_DEVINL void request(int c, int NC) {       // a chunk outside the sequence: nothing is read
         const bool inside = c >= 0 && c < NC;
@@ -436,18 +445,35 @@ struct ChunkRows {
             kn[p] = kc.raw(row, col);
             if (TWO) qn[p] = qc.raw(row, col);
         }
+        if (AHEAD) {
+            const ChunkBase ac = chunk_base(a + (int64_t)c * BLK * NA * BFRAG, A_BYTES, inside), bc = chunk_base(b + (int64_t)c * BLK * NB * BFRAG, B_BYTES, inside);
+#pragma unroll
+            for (int x = 0; x < NX; ++x) {
+                const int kb = x * W + wave;      // a kilobyte of one of the two per wave and step
+                if (kb < A_BYTES / 1024) xn[x] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ac.r, kb * 1024 + (tid & 63) * 16, 0, 0));
+                else if (kb < KBS) xn[x] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(bc.r, kb * 1024 - A_BYTES + (tid & 63) * 16, 0, 0));
+            }
+        }
         if (tid < DC) {
             bn = tid < left ? beta[((int64_t)c * DC + tid) * H] : 0.f;
             gn = gam[(int64_t)c * 2 * DC + tid];  // (chunk 0's instead)
             en = gam[(int64_t)c * 2 * DC + DC + tid];
         }
     }
-    VA_DEVINL void place(char* lds) {
+    VA_DEVINL void place(char* lds, int c) {
 #pragma unroll
         for (int p = 0; p < N; ++p) {
             const int idx = p * 64 * W + tid, at = quad_at<HD>(idx / (HD / 4), idx % (HD / 4));
             put_rows(lds + at, DC * HD * 2, kn[p]);
             if (TWO) put_rows(lds + MATRIX + at, DC * HD * 2, qn[p]);
+        }
+        if (AHEAD) {                              // the two operands lie one behind the other
+#pragma unroll
+            for (int x = 0; x < NX; ++x)
+                if (x * W + wave < KBS) *(u32x4_t*)(lds + A_AT + (x * W + wave) * 1024 + (tid & 63) * 16) = xn[x];
+        } else {
+            to_lds<A_BYTES, W>(a + (int64_t)c * BLK * NA * BFRAG, lds + A_AT, wave, tid & 63);
+            if (NB > 0) to_lds<B_BYTES, W>(b + (int64_t)c * BLK * NB * BFRAG, lds + B_AT, wave, tid & 63);
         }
         float* f = (float*)(lds + F_AT);
         if (tid < DC) f[tid] = bn, f[DC + tid] = gn, f[2 * DC + tid] = en;
@@ -480,8 +506,7 @@ VA_DEVINL void rows_times(const char* x, int u, const bf16x8_t (&b)[CG][NB], f32
 
 // ---------------------------------------------------------------------------------------------------------------
 // The sequential part.  A wave owns 16 CG columns (values of the head) of the state for the whole sequence: M in CG * HD/16
-// accumulator tiles; W waves share a chunk's K, Q, T and P through LDS.  K and Q of the next chunk are requested half-way
-// through the current one, T and P of a chunk arrive while its products with M are formed.
+// accumulator tiles; W waves share a chunk's K, Q, T and P through LDS, the next chunk's are requested while one computes.
 // OUT: writes o.  SAVE: writes U and every chunk's starting state (rows of S) for the gradient.
 template <int HD, typename T, int W, int CG, bool OUT, bool SAVE>
 __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
@@ -491,10 +516,10 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
                                                             T* __restrict__ O, float* __restrict__ STATE_OUT,
                                                             float* __restrict__ US, float* __restrict__ MS, int L, int H, int NC) {
     constexpr int NI = parts<T>::IN, NM = parts<T>::MID, NO = parts<T>::OUT;
-    typedef ChunkRows<HD, T, W, OUT, NM, OUT ? NO : 0> CR;
+    typedef ChunkRows<HD, T, W, OUT, NM, OUT ? NO : 0, CG == 1> CR;
     extern __shared__ __align__(16) char lds[];
     const char *ks = lds, *qs = lds + CR::MATRIX;
-    char *tl = lds + CR::A_AT, *pl = lds + CR::B_AT;
+    const char *tl = lds + CR::A_AT, *pl = lds + CR::B_AT;
     const float *sb = (const float*)(lds + CR::F_AT), *sg = sb + DC, *se = sg + DC;
     constexpr int GROUPS = HD / 16 / (W * CG);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4, g4 = g * 4;
@@ -504,7 +529,8 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
     const T* vb = V + rv.at(b, L, 0, h, HD);
     CR cr;
     cr.k = K + rk.at(b, L, 0, h, HD), cr.q = Q + rq.at(b, L, 0, h, HD), cr.ldk = rk.ld, cr.ldq = rq.ld;
-    cr.beta = BETA + b * L * H + h, cr.gam = GAM + bh * NC * 2 * DC, cr.L = L, cr.H = H, cr.tid = tid;
+    cr.beta = BETA + b * L * H + h, cr.gam = GAM + bh * NC * 2 * DC, cr.L = L, cr.H = H, cr.tid = tid, cr.wave = wave;
+    cr.a = TF + bh * NC * BLK * NM * BFRAG, cr.b = PF + bh * NC * BLK * NO * BFRAG;
     f32x4_t M[CG][HD / 16];
 #pragma unroll
     for (int x = 0; x < CG; ++x)
@@ -518,9 +544,7 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
         const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
         const int64_t ci = bh * NC + c;
         __syncthreads();                          // everybody is done with the chunk before
-        cr.place(lds);
-        to_lds<CR::A_BYTES, W>(TF + ci * BLK * NM * BFRAG, tl, wave, lane);
-        if (OUT) to_lds<CR::B_BYTES, W>(PF + ci * BLK * NO * BFRAG, pl, wave, lane);
+        cr.place(lds, c);
         f32x4_t vv[CG][4];                        // this chunk's v columns, rows in accumulator order
         const ChunkOf<T> vc = chunk_of(vb + (int64_t)t0 * rv.ld, rv.ld, left);
 #pragma unroll
@@ -530,6 +554,7 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
 #pragma unroll
                 for (int r = 0; r < 4; ++r) vv[x][it][r] = vc.get(16 * it + g4 + r, v + 16 * x);
         lds_barrier();
+        if (CG == 1) cr.request(c + 1, NC);
         f32x4_t rhs[CG][4], o[CG][4], U[CG][4];
 #pragma unroll
         for (int x = 0; x < CG; ++x) {
@@ -569,9 +594,11 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
             split(rhs[x][0], rhs[x][1], f0[x]);
             split(rhs[x][2], rhs[x][3], f1[x]);
         }
-        wait_vm0();
-        __syncthreads();                          // T and P are there
-        cr.request(c + 1, NC);
+        if (CG > 1) {
+            wait_vm0();
+            __syncthreads();                      // T and P are there
+            cr.request(c + 1, NC);
+        }
         blocks_times<4, false, NM>(tl, 0, 0, f0, U, lane);
         blocks_times<2, false, NM>(tl, 2, 1, f1, U, lane);
         if (SAVE) {
@@ -629,10 +656,10 @@ __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict
                                                              T* __restrict__ DV, float* __restrict__ DSTATE_IN,
                                                              float* __restrict__ RS, float* __restrict__ GS, int L, int H, int NC) {
     constexpr int NI = parts<T>::IN, NM = parts<T>::MID;
-    typedef ChunkRows<HD, T, W, true, NM, NM> CR;
+    typedef ChunkRows<HD, T, W, true, NM, NM, CG == 1> CR;
     extern __shared__ __align__(16) char lds[];
     const char *ks = lds, *qs = lds + CR::MATRIX;
-    char *pl = lds + CR::A_AT, *tl = lds + CR::B_AT;
+    const char *pl = lds + CR::A_AT, *tl = lds + CR::B_AT;
     const float *sb = (const float*)(lds + CR::F_AT), *sg = sb + DC, *se = sg + DC;
     constexpr int GROUPS = HD / 16 / (W * CG);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4, g4 = g * 4;
@@ -641,7 +668,8 @@ __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict
     const int v = ((wid % GROUPS) * W + wave) * 16 * CG + m;
     CR cr;
     cr.k = K + rk.at(b, L, 0, h, HD), cr.q = Q + rq.at(b, L, 0, h, HD), cr.ldk = rk.ld, cr.ldq = rq.ld;
-    cr.beta = BETA + b * L * H + h, cr.gam = GAM + bh * NC * 2 * DC, cr.L = L, cr.H = H, cr.tid = tid;
+    cr.beta = BETA + b * L * H + h, cr.gam = GAM + bh * NC * 2 * DC, cr.L = L, cr.H = H, cr.tid = tid, cr.wave = wave;
+    cr.a = PT + bh * NC * BLK * NM * BFRAG, cr.b = TT + bh * NC * BLK * NM * BFRAG;
     f32x4_t G[CG][HD / 16];
 #pragma unroll
     for (int x = 0; x < CG; ++x)
@@ -655,9 +683,7 @@ __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict
         const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
         const int64_t ci = bh * NC + c;
         __syncthreads();                          // everybody is done with the chunk before
-        cr.place(lds);
-        to_lds<CR::A_BYTES, W>(PT + ci * BLK * NM * BFRAG, pl, wave, lane);
-        to_lds<CR::B_BYTES, W>(TT + ci * BLK * NM * BFRAG, tl, wave, lane);
+        cr.place(lds, c);
         f32x4_t dov[CG][4];
         const ChunkOf<T> oc = chunk_of(DO + ((b * L + t0) * H + h) * HD, (int64_t)H * HD, left);
 #pragma unroll
@@ -667,6 +693,7 @@ __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict
 #pragma unroll
                 for (int r = 0; r < 4; ++r) dov[x][it][r] = oc.get(16 * it + g4 + r, v + 16 * x);
         lds_barrier();
+        if (CG == 1) cr.request(c - 1, NC);
         f32x4_t du[CG][4], R[CG][4];
 #pragma unroll
         for (int x = 0; x < CG; ++x) {
@@ -690,9 +717,11 @@ __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict
             split(dov[x][0], dov[x][1], o0[x]);
             split(dov[x][2], dov[x][3], o1[x]);
         }
-        wait_vm0();
-        __syncthreads();                          // P^T and T^T are there
-        cr.request(c - 1, NC);
+        if (CG > 1) {
+            wait_vm0();
+            __syncthreads();                      // P^T and T^T are there
+            cr.request(c - 1, NC);
+        }
         blocks_times<2, true, NM>(pl, 0, 0, o0, du, lane);
         blocks_times<4, true, NM>(pl, 0, 1, o1, du, lane);
 #pragma unroll
@@ -1113,11 +1142,30 @@ struct Pieces {
     }
 };
 
-template <int HD, typename T, bool GRAD>
-int launch_prep(const DeltaArgs& d, bf16_t* tf, bf16_t* tt, bf16_t* pf, float* gam, hipStream_t stream) {
-    hipLaunchKernelGGL((delta_prep_kernel<HD, T, GRAD>), dim3((unsigned)(d.B * d.H * d.chunks())), dim3(256), 0, stream, (const T*)d.q,
-                       (const T*)d.k, Rows{d.ldq}, Rows{d.ldk}, d.alpha, d.beta, tf, tt, pf, gam, (int)d.L, (int)d.H,
-                       (int)d.chunks());
+// What a forward pass leaves for its gradient, and what it needs itself
+template <typename T> struct Work {
+    bf16_t *tf, *pf, *tt, *pt;
+    float *gam, *us, *ms;
+};
+template <typename T> int64_t operand_numbers(const DeltaArgs& d, int parts_) { return d.B * d.H * d.chunks() * BLK * BFRAG * parts_; }
+template <typename T> void take_own(const DeltaArgs& d, Pieces& p, Work<T>& w) {
+    w.tf = p.template take<bf16_t>(operand_numbers<T>(d, parts<T>::MID));
+    w.pf = p.template take<bf16_t>(operand_numbers<T>(d, parts<T>::OUT));
+}
+template <typename T> void take_kept(const DeltaArgs& d, Pieces& p, Work<T>& w) {
+    const int64_t n = d.B * d.H * d.chunks();
+    w.gam = p.template take<float>(n * 2 * DC);
+    w.tt = p.template take<bf16_t>(operand_numbers<T>(d, parts<T>::MID));
+    w.pt = p.template take<bf16_t>(operand_numbers<T>(d, parts<T>::MID));
+    w.us = p.template take<float>(n * DC * d.hd);
+    w.ms = p.template take<float>(n * d.hd * d.hd);
+}
+
+template <int HD, typename T, bool TRAIN>
+int launch_prep(const DeltaArgs& d, const Work<T>& w, hipStream_t stream) {
+    hipLaunchKernelGGL((delta_prep_kernel<HD, T, TRAIN>), dim3((unsigned)(d.B * d.H * d.chunks())), dim3(256), 0, stream,
+                       (const T*)d.q, (const T*)d.k, Rows{d.ldq}, Rows{d.ldk}, d.alpha, d.beta, w.tf, w.pf, w.tt, w.pt, w.gam,
+                       (int)d.L, (int)d.H, (int)d.chunks());
     VA_CHECK_LAUNCH("va_gated_delta (decays)");
     return VA_OK;
 }
@@ -1129,69 +1177,80 @@ constexpr int SCAN_W = 4;
 template <int HD> bool wide_scan(const DeltaArgs& d) { return HD == 128 && d.B * d.H > 128; }
 
 template <int HD, typename T, int CG, bool OUT, bool SAVE>
-int launch_scan(const DeltaArgs& d, const bf16_t* tf, const bf16_t* pf, const float* gam, const float* state_in, void* out,
-                float* state_out, float* us, float* ms, hipStream_t stream) {
-    constexpr int lds = ChunkRows<HD, T, SCAN_W, OUT, parts<T>::MID, OUT ? parts<T>::OUT : 0>::LDS;
+int launch_scan(const DeltaArgs& d, const Work<T>& w, const float* state_in, void* out, float* state_out, hipStream_t stream) {
+    constexpr int lds = ChunkRows<HD, T, SCAN_W, OUT, parts<T>::MID, OUT ? parts<T>::OUT : 0, CG == 1>::LDS;
     const auto fn = delta_scan_kernel<HD, T, SCAN_W, CG, OUT, SAVE>;
     VA_TRY(reserve_lds("va_gated_delta", (const void*)fn, lds));
     hipLaunchKernelGGL(fn, dim3((unsigned)(d.B * d.H * (HD / 16 / (SCAN_W * CG)))), dim3(64 * SCAN_W), lds, stream, (const T*)d.q,
-                       (const T*)d.k, (const T*)d.v, Rows{d.ldq}, Rows{d.ldk}, Rows{d.ldv}, d.beta, tf, pf, gam, state_in, (T*)out,
-                       state_out, us, ms, (int)d.L, (int)d.H, (int)d.chunks());
+                       (const T*)d.k, (const T*)d.v, Rows{d.ldq}, Rows{d.ldk}, Rows{d.ldv}, d.beta, w.tf, w.pf, w.gam, state_in,
+                       (T*)out, state_out, w.us, w.ms, (int)d.L, (int)d.H, (int)d.chunks());
     VA_CHECK_LAUNCH("va_gated_delta (scan)");
     return VA_OK;
 }
+template <int HD, typename T, bool OUT, bool SAVE>
+int run_scan(const DeltaArgs& d, const Work<T>& w, const float* state_in, void* out, float* state_out, hipStream_t stream) {
+    if (wide_scan<HD>(d)) return launch_scan<HD, T, HD / 64, OUT, SAVE>(d, w, state_in, out, state_out, stream);
+    return launch_scan<HD, T, 1, OUT, SAVE>(d, w, state_in, out, state_out, stream);
+}
 
 template <int HD, typename T, int CG>
-int launch_rscan(const DeltaArgs& d, const void* d_out, const bf16_t* tt, const bf16_t* pt, const float* gam, const float* d_state,
-                 void* dv, float* d_state_in, float* rs, float* gs, hipStream_t stream) {
-    constexpr int lds = ChunkRows<HD, T, SCAN_W, true, parts<T>::MID, parts<T>::MID>::LDS;
+int launch_rscan(const DeltaArgs& d, const Work<T>& w, const void* d_out, const float* d_state, void* dv, float* d_state_in, float* rs,
+                 float* gs, hipStream_t stream) {
+    constexpr int lds = ChunkRows<HD, T, SCAN_W, true, parts<T>::MID, parts<T>::MID, CG == 1>::LDS;
     const auto fn = delta_rscan_kernel<HD, T, SCAN_W, CG>;
     VA_TRY(reserve_lds("va_gated_delta_bwd", (const void*)fn, lds));
     hipLaunchKernelGGL(fn, dim3((unsigned)(d.B * d.H * (HD / 16 / (SCAN_W * CG)))), dim3(64 * SCAN_W), lds, stream, (const T*)d.q,
-                       (const T*)d.k, Rows{d.ldq}, Rows{d.ldk}, (const T*)d_out, d.beta, tt, pt, gam, d_state, (T*)dv, d_state_in, rs,
-                       gs, (int)d.L, (int)d.H, (int)d.chunks());
+                       (const T*)d.k, Rows{d.ldq}, Rows{d.ldk}, (const T*)d_out, d.beta, w.tt, w.pt, w.gam, d_state, (T*)dv, d_state_in,
+                       rs, gs, (int)d.L, (int)d.H, (int)d.chunks());
     VA_CHECK_LAUNCH("va_gated_delta_bwd (scan)");
     return VA_OK;
 }
 
-// bytes of one chunk's share of a workspace
+// bytes of one chunk's share of the forward's own workspace, of what it keeps, and of the gradient's own
 constexpr int64_t OPERAND_BYTES = BLK * BFRAG * 2;
-int64_t fwd_chunk_bytes() { return 6 * OPERAND_BYTES + 2 * DC * 4; }
-int64_t bwd_chunk_bytes(int64_t hd) { return 9 * OPERAND_BYTES + 2 * DC * 4 + 2 * DC * hd * 4 + 2 * hd * hd * 4; }
+int64_t own_chunk_bytes() { return 6 * OPERAND_BYTES + 2 * DC * 4; }
+int64_t kept_chunk_bytes(int64_t hd) { return 2 * DC * 4 + 6 * OPERAND_BYTES + DC * hd * 4 + hd * hd * 4; }
+int64_t bwd_chunk_bytes(int64_t hd) { return DC * hd * 4 + hd * hd * 4; }
 
 template <int HD, typename T>
-int delta_fwd(const DeltaArgs& d, const float* state_in, void* out, float* state_out, float* ws, hipStream_t stream) {
-    const int64_t n = d.B * d.H * d.chunks();
-    Pieces w = {(char*)ws};
-    bf16_t* tf = w.take<bf16_t>(n * BLK * BFRAG * parts<T>::MID);
-    bf16_t* pf = w.take<bf16_t>(n * BLK * BFRAG * parts<T>::OUT);
-    float* gam = w.take<float>(n * 2 * DC);
-    VA_TRY((launch_prep<HD, T, false>(d, tf, nullptr, pf, gam, stream)));
-    if (wide_scan<HD>(d)) return launch_scan<HD, T, HD / 64, true, false>(d, tf, pf, gam, state_in, out, state_out, nullptr, nullptr, stream);
-    return launch_scan<HD, T, 1, true, false>(d, tf, pf, gam, state_in, out, state_out, nullptr, nullptr, stream);
+int delta_fwd(const DeltaArgs& d, const float* state_in, void* out, float* state_out, float* ws, float* kept, hipStream_t stream) {
+    Work<T> w = {};
+    Pieces own = {(char*)ws};
+    take_own(d, own, w);
+    if (kept != nullptr) {
+        Pieces k = {(char*)kept};
+        take_kept(d, k, w);
+        VA_TRY((launch_prep<HD, T, true>(d, w, stream)));
+        return run_scan<HD, T, true, true>(d, w, state_in, out, state_out, stream);
+    }
+    w.gam = own.template take<float>(d.B * d.H * d.chunks() * 2 * DC);
+    VA_TRY((launch_prep<HD, T, false>(d, w, stream)));
+    return run_scan<HD, T, true, false>(d, w, state_in, out, state_out, stream);
 }
 
 template <int HD, typename T>
 int delta_bwd(const DeltaArgs& d, const void* d_out, const float* d_state, const float* state_in, void* dq, void* dk, void* dv,
-              float* dalpha, float* dbeta, float* d_state_in, float* ws, hipStream_t stream) {
-    const int64_t n = d.B * d.H * d.chunks(), ops = n * BLK * BFRAG * parts<T>::MID;
-    Pieces w = {(char*)ws};
-    bf16_t *tf = w.take<bf16_t>(ops), *tt = w.take<bf16_t>(ops), *pt = w.take<bf16_t>(ops);
-    float *gam = w.take<float>(n * 2 * DC), *us = w.take<float>(n * DC * HD), *rs = w.take<float>(n * DC * HD);
-    float *ms = w.take<float>(n * HD * HD), *gs = w.take<float>(n * HD * HD);
-    VA_TRY((launch_prep<HD, T, true>(d, tf, tt, pt, gam, stream)));
-    if (wide_scan<HD>(d)) {
-        VA_TRY((launch_scan<HD, T, HD / 64, false, true>(d, tf, nullptr, gam, state_in, nullptr, nullptr, us, ms, stream)));
-        VA_TRY((launch_rscan<HD, T, HD / 64>(d, d_out, tt, pt, gam, d_state, dv, d_state_in, rs, gs, stream)));
+              float* dalpha, float* dbeta, float* d_state_in, float* ws, const float* kept, hipStream_t stream) {
+    const int64_t n = d.B * d.H * d.chunks();
+    Work<T> w = {};
+    Pieces own = {(char*)ws};
+    float *rs = own.take<float>(n * DC * HD), *gs = own.take<float>(n * HD * HD);
+    if (kept != nullptr) {
+        Pieces k = {(char*)kept};
+        take_kept(d, k, w);
     } else {
-        VA_TRY((launch_scan<HD, T, 1, false, true>(d, tf, nullptr, gam, state_in, nullptr, nullptr, us, ms, stream)));
-        VA_TRY((launch_rscan<HD, T, 1>(d, d_out, tt, pt, gam, d_state, dv, d_state_in, rs, gs, stream)));
+        take_kept(d, own, w);
+        take_own(d, own, w);
+        VA_TRY((launch_prep<HD, T, true>(d, w, stream)));
+        VA_TRY((run_scan<HD, T, false, true>(d, w, state_in, nullptr, nullptr, stream)));
     }
+    if (wide_scan<HD>(d)) VA_TRY((launch_rscan<HD, T, HD / 64>(d, w, d_out, d_state, dv, d_state_in, rs, gs, stream)));
+    else VA_TRY((launch_rscan<HD, T, 1>(d, w, d_out, d_state, dv, d_state_in, rs, gs, stream)));
     constexpr int lds = (2 * DC * (HD + 4) + 4 * DC * SQ + 3 * DC + 4 * DC + 12 * DC + DC + 4 + 2 * DC) * 4;
     const auto fn = delta_grad_kernel<HD, T>;
     VA_TRY(reserve_lds("va_gated_delta_bwd", (const void*)fn, lds));
     hipLaunchKernelGGL(fn, dim3((unsigned)n), dim3(256), lds, stream, (const T*)d.q, (const T*)d.k, (const T*)d.v, Rows{d.ldq},
-                       Rows{d.ldk}, Rows{d.ldv}, (const T*)d_out, d.alpha, d.beta, us, rs, ms, gs, (T*)dq, (T*)dk, dalpha, dbeta,
+                       Rows{d.ldk}, Rows{d.ldv}, (const T*)d_out, d.alpha, d.beta, w.us, rs, w.ms, gs, (T*)dq, (T*)dk, dalpha, dbeta,
                        (int)d.L, (int)d.H, (int)d.chunks());
     VA_CHECK_LAUNCH("va_gated_delta_bwd (gradients)");
     return VA_OK;
@@ -1199,46 +1258,51 @@ int delta_bwd(const DeltaArgs& d, const void* d_out, const float* d_state, const
 
 }  // namespace
 
-extern "C" int64_t va_gated_delta_fwd_workspace_floats(int64_t B, int64_t L, int64_t H, int64_t hd) {
+static int64_t delta_floats(int64_t B, int64_t L, int64_t H, int64_t hd, int64_t chunk_bytes) {
     if (B <= 0 || L <= 0 || H <= 0 || (hd != 64 && hd != 128)) return 0;
-    return B * H * ((L + DC - 1) / DC) * fwd_chunk_bytes() / 4;
+    return B * H * ((L + DC - 1) / DC) * chunk_bytes / 4;
 }
-
-extern "C" int64_t va_gated_delta_bwd_workspace_floats(int64_t B, int64_t L, int64_t H, int64_t hd) {
-    if (B <= 0 || L <= 0 || H <= 0 || (hd != 64 && hd != 128)) return 0;
-    return B * H * ((L + DC - 1) / DC) * bwd_chunk_bytes(hd) / 4;
+extern "C" int64_t va_gated_delta_fwd_workspace_floats(int64_t B, int64_t L, int64_t H, int64_t hd) {
+    return delta_floats(B, L, H, hd, own_chunk_bytes());
+}
+extern "C" int64_t va_gated_delta_kept_floats(int64_t B, int64_t L, int64_t H, int64_t hd) {
+    return delta_floats(B, L, H, hd, kept_chunk_bytes(hd));
+}
+extern "C" int64_t va_gated_delta_bwd_workspace_floats(int64_t B, int64_t L, int64_t H, int64_t hd, int have_kept) {
+    return delta_floats(B, L, H, hd, bwd_chunk_bytes(hd) + (have_kept ? 0 : own_chunk_bytes() + kept_chunk_bytes(hd)));
 }
 
 extern "C" int va_gated_delta_fwd(const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv, int is_bf16,
                                   const float* alpha, const float* beta, const float* state_in, void* out, float* state_out,
-                                  float* workspace, int64_t B, int64_t L, int64_t H, int64_t hd, hipStream_t stream) {
+                                  float* workspace, float* kept, int64_t B, int64_t L, int64_t H, int64_t hd, hipStream_t stream) {
     const DeltaArgs d = {q, k, v, ldq, ldk, ldv, alpha, beta, B, L, H, hd, is_bf16 != 0};
     VA_TRY(delta_check("va_gated_delta_fwd", d));
     VA_CHECK_ARG(out && state_out && workspace, "va_gated_delta_fwd: null operand");
-    VA_CHECK_ARG(((uintptr_t)state_in | (uintptr_t)state_out | (uintptr_t)workspace) % 16 == 0,
+    VA_CHECK_ARG(((uintptr_t)state_in | (uintptr_t)state_out | (uintptr_t)workspace | (uintptr_t)kept) % 16 == 0,
                  "va_gated_delta_fwd: misaligned state or workspace");
     if (hd == 128)
-        return d.bf16 ? delta_fwd<128, bf16_t>(d, state_in, out, state_out, workspace, stream)
-                      : delta_fwd<128, float>(d, state_in, out, state_out, workspace, stream);
-    return d.bf16 ? delta_fwd<64, bf16_t>(d, state_in, out, state_out, workspace, stream)
-                  : delta_fwd<64, float>(d, state_in, out, state_out, workspace, stream);
+        return d.bf16 ? delta_fwd<128, bf16_t>(d, state_in, out, state_out, workspace, kept, stream)
+                      : delta_fwd<128, float>(d, state_in, out, state_out, workspace, kept, stream);
+    return d.bf16 ? delta_fwd<64, bf16_t>(d, state_in, out, state_out, workspace, kept, stream)
+                  : delta_fwd<64, float>(d, state_in, out, state_out, workspace, kept, stream);
 }
 
 extern "C" int va_gated_delta_bwd(const void* d_out, const float* d_state, const void* q, const void* k, const void* v, int64_t ldq,
                                   int64_t ldk, int64_t ldv, int is_bf16, const float* alpha, const float* beta,
                                   const float* state_in, void* dq, void* dk, void* dv, float* dalpha, float* dbeta,
-                                  float* d_state_in, float* workspace, int64_t B, int64_t L, int64_t H, int64_t hd,
+                                  float* d_state_in, float* workspace, const float* kept, int64_t B, int64_t L, int64_t H, int64_t hd,
                                   hipStream_t stream) {
     const DeltaArgs d = {q, k, v, ldq, ldk, ldv, alpha, beta, B, L, H, hd, is_bf16 != 0};
     VA_TRY(delta_check("va_gated_delta_bwd", d));
     VA_CHECK_ARG(d_out && dq && dk && dv && dalpha && dbeta && workspace, "va_gated_delta_bwd: null operand");
-    VA_CHECK_ARG(((uintptr_t)state_in | (uintptr_t)d_state | (uintptr_t)d_state_in | (uintptr_t)workspace | (uintptr_t)d_out) % 16 == 0,
+    VA_CHECK_ARG(((uintptr_t)state_in | (uintptr_t)d_state | (uintptr_t)d_state_in | (uintptr_t)workspace | (uintptr_t)kept |
+                  (uintptr_t)d_out) % 16 == 0,
                  "va_gated_delta_bwd: misaligned state, gradient or workspace");
     if (hd == 128)
-        return d.bf16 ? delta_bwd<128, bf16_t>(d, d_out, d_state, state_in, dq, dk, dv, dalpha, dbeta, d_state_in, workspace, stream)
-                      : delta_bwd<128, float>(d, d_out, d_state, state_in, dq, dk, dv, dalpha, dbeta, d_state_in, workspace, stream);
-    return d.bf16 ? delta_bwd<64, bf16_t>(d, d_out, d_state, state_in, dq, dk, dv, dalpha, dbeta, d_state_in, workspace, stream)
-                  : delta_bwd<64, float>(d, d_out, d_state, state_in, dq, dk, dv, dalpha, dbeta, d_state_in, workspace, stream);
+        return d.bf16 ? delta_bwd<128, bf16_t>(d, d_out, d_state, state_in, dq, dk, dv, dalpha, dbeta, d_state_in, workspace, kept, stream)
+                      : delta_bwd<128, float>(d, d_out, d_state, state_in, dq, dk, dv, dalpha, dbeta, d_state_in, workspace, kept, stream);
+    return d.bf16 ? delta_bwd<64, bf16_t>(d, d_out, d_state, state_in, dq, dk, dv, dalpha, dbeta, d_state_in, workspace, kept, stream)
+                  : delta_bwd<64, float>(d, d_out, d_state, state_in, dq, dk, dv, dalpha, dbeta, d_state_in, workspace, kept, stream);
 }
 
 extern "C" int va_gated_delta_step(const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv, int is_bf16,

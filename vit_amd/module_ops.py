@@ -235,19 +235,22 @@ class GatedDeltaFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, alpha, beta, state):
         args = [None if t is None else t.detach() for t in (q, k, v, alpha, beta, state)]
-        out, new_state = ops.gated_delta_fwd(*args)
-        ctx.save_for_backward(q, k, v, alpha, beta, state)
+        if not any(ctx.needs_input_grad):
+            return ops.gated_delta_fwd(*args)
+        out, new_state, kept = ops.gated_delta_fwd(*args, keep=True)
+        ctx.save_for_backward(q, k, v, alpha, beta, state, kept)
         ctx.set_materialize_grads(False)
         return out, new_state
 
     @staticmethod
     def backward(ctx, d_out, d_state):
-        q, k, v, alpha, beta, state = ctx.saved_tensors
+        q, k, v, alpha, beta, state, kept = ctx.saved_tensors
         if d_out is None and d_state is None:
             return (None,) * 6
         d_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if d_out is None else d_out.contiguous()
         want = state is not None and ctx.needs_input_grad[5]
-        grads = ops.gated_delta_bwd(d_out, None if d_state is None else d_state.contiguous(), q, k, v, alpha, beta, state, want)
+        grads = ops.gated_delta_bwd(d_out, None if d_state is None else d_state.contiguous(), q, k, v, alpha, beta, state, want,
+                                    kept)
         return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad))
 
 

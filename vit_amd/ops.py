@@ -603,24 +603,27 @@ def _delta_operands(who: str, q, k, v, alpha, beta, state, lead: int):
     return _heads_ld(q, "q"), _heads_ld(k, "k"), _heads_ld(v, "v")
 
 
-def gated_delta_fwd(q, k, v, alpha, beta, state=None):
+def gated_delta_fwd(q, k, v, alpha, beta, state=None, keep: bool = False):
     """The recurrence of `gated_delta_seq` in its chunked form (products over 64 tokens on the matrix pipe): q, k, v f32 or
     bf16 [B,L,H,hd] (rows any constant stride apart), hd 64 or 128; alpha, beta f32 [B,L,H]; state f32 [B,H,hd,hd] or None
-    -> (out [B,L,H,hd] of q's type, new state f32).  A non-finite token spreads over its chunk of 64."""
+    -> (out [B,L,H,hd] of q's type, new state f32).  A non-finite token spreads over its chunk of 64.  keep=True: a third
+    result, what `gated_delta_bwd` otherwise computes again (about 2 KiB per token and head of 128)."""
     lds = _delta_operands("gated_delta_fwd", q, k, v, alpha, beta, state, 2)
     B, L, H, hd = q.shape
     lib = _lib.load()
     out = torch.empty(B, L, H, hd, dtype=q.dtype, device=q.device)
     new_state = torch.empty(B, H, hd, hd, dtype=F32, device=q.device)
     ws = torch.empty(lib.va_gated_delta_fwd_workspace_floats(B, L, H, hd), dtype=F32, device=q.device)
+    kept = torch.empty(lib.va_gated_delta_kept_floats(B, L, H, hd), dtype=F32, device=q.device) if keep else None
     check(lib.va_gated_delta_fwd(_p(q), _p(k), _p(v), *lds, int(q.dtype == BF16), _p(alpha), _p(beta), _p(state), _p(out),
-                                 _p(new_state), _p(ws), B, L, H, hd, _stream()), "va_gated_delta_fwd")
-    return out, new_state
+                                 _p(new_state), _p(ws), _p(kept), B, L, H, hd, _stream()), "va_gated_delta_fwd")
+    return (out, new_state, kept) if keep else (out, new_state)
 
 
-def gated_delta_bwd(d_out, d_state, q, k, v, alpha, beta, state=None, want_state: bool = True):
+def gated_delta_bwd(d_out, d_state, q, k, v, alpha, beta, state=None, want_state: bool = True, kept=None):
     """Gradients of `gated_delta_fwd`: d_out as out, d_state (of the final state) f32 or None -> (dq, dk, dv of q's type,
-    dalpha, dbeta f32, gradient of the initial state f32 or None).  Takes the forward's inputs; recomputes the rest."""
+    dalpha, dbeta f32, gradient of the initial state f32 or None).  Takes the forward's inputs, and `kept` if it was called
+    with keep=True."""
     lds = _delta_operands("gated_delta_bwd", q, k, v, alpha, beta, state, 2)
     B, L, H, hd = q.shape
     _need(d_out, q.dtype, "d_out")
@@ -634,10 +637,14 @@ def gated_delta_bwd(d_out, d_state, q, k, v, alpha, beta, state=None, want_state
     dq, dk, dv = (torch.empty(B, L, H, hd, dtype=q.dtype, device=q.device) for _ in range(3))
     da, db = torch.empty_like(alpha), torch.empty_like(beta)
     ds = torch.empty(B, H, hd, hd, dtype=F32, device=q.device) if want_state else None
-    ws = torch.empty(lib.va_gated_delta_bwd_workspace_floats(B, L, H, hd), dtype=F32, device=q.device)
+    if kept is not None:
+        _need(kept, F32, "kept")
+        if kept.numel() != lib.va_gated_delta_kept_floats(B, L, H, hd) or not kept.is_contiguous():
+            raise ValueError("gated_delta_bwd: kept does not belong to a forward of these sizes")
+    ws = torch.empty(lib.va_gated_delta_bwd_workspace_floats(B, L, H, hd, int(kept is not None)), dtype=F32, device=q.device)
     check(lib.va_gated_delta_bwd(_p(d_out), _p(d_state), _p(q), _p(k), _p(v), *lds, int(q.dtype == BF16), _p(alpha), _p(beta),
-                                 _p(state), _p(dq), _p(dk), _p(dv), _p(da), _p(db), _p(ds), _p(ws), B, L, H, hd, _stream()),
-          "va_gated_delta_bwd")
+                                 _p(state), _p(dq), _p(dk), _p(dv), _p(da), _p(db), _p(ds), _p(ws), _p(kept), B, L, H, hd,
+                                 _stream()), "va_gated_delta_bwd")
     return dq, dk, dv, da, db, ds
 
 
