@@ -178,12 +178,12 @@ VA_DEVINL float chunk_prefix(float mine, int lane) {
     return p;
 }
 
-template <int HD, typename T>
+template <int HD, typename T, int THREADS>
 VA_DEVINL void rows_to_lds(const ChunkOf<T>& src, float (*dst)[HD + 4], int tid) {
-    constexpr int N = DC * HD / 4 / 256;
+    constexpr int N = DC * HD / 4 / THREADS;
 #pragma unroll
     for (int p = 0; p < N; ++p) {
-        const int idx = p * 256 + tid, row = idx / (HD / 4), c = (idx % (HD / 4)) * 4;
+        const int idx = p * THREADS + tid, row = idx / (HD / 4), c = (idx % (HD / 4)) * 4;
         *(f32x4_t*)&dst[row][c] = widen4(src.raw(row, c));
     }
 }
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q
     const int64_t ci = (b * H + h) * NC + c;
     const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
     const ChunkOf<T> qc = chunk_of(Q + rq.at(b, L, t0, h, HD), rq.ld, left);
-    rows_to_lds<HD, T>(chunk_of(K + rk.at(b, L, t0, h, HD), rk.ld, left), ks, tid);
+    rows_to_lds<HD, T, 256>(chunk_of(K + rk.at(b, L, t0, h, HD), rk.ld, left), ks, tid);
     const float mine = lane < left ? ALPHA[(b * L + t0 + lane) * H + h] : 1.0f;
     if (tid < DC) sb[tid] = tid < left ? BETA[(b * L + t0 + tid) * H + h] : 0.0f;
     if (wave == 0) chunk_decays(mine, gt, lane);
@@ -482,16 +482,16 @@ struct ChunkRows {
 
 // acc[c][ct] += X^T B for all HD/16 column tiles of X, B (token blocks u) in parts
 template <int HD, int NX, int NB, int CG>
-VA_DEVINL void columns_times(const char* x, const bf16x8_t (&b0)[CG][NB], const bf16x8_t (&b1)[CG][NB], f32x4_t (&acc)[CG][HD / 16],
+VA_DEVINL void columns_times(const char* x_, const bf16x8_t (&b0)[CG][NB], const bf16x8_t (&b1)[CG][NB], f32x4_t (&acc)[CG][HD / 16],
                              int lane) {
 #pragma unroll
-    for (int ct = 0; ct < HD / 16; ct += 2) {
-        bf16x8_t a[2][NX];
-        col_frag<HD>(x, ct, 0, lane, a[0]);
-        col_frag<HD>(x, ct + 1, 0, lane, a[1]);
+    for (int ct = 0; ct < HD / 16; ct += 4) {
+        bf16x8_t a[4][NX];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) col_frag<HD>(x_, ct + x, 0, lane, a[x]);
         mfma_parts(a, b0, acc, ct);
-        col_frag<HD>(x, ct, 1, lane, a[0]);
-        col_frag<HD>(x, ct + 1, 1, lane, a[1]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) col_frag<HD>(x_, ct + x, 1, lane, a[x]);
         mfma_parts(a, b1, acc, ct);
     }
 }
@@ -770,47 +770,54 @@ __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// What is left of the gradient, chunk by chunk in parallel.  Wave w owns all 64 rows of columns [w HD/4, (w+1) HD/4) of
-// dQ and dK, so a chunk's M and G are read once; the 64x64 matrices are formed tile by tile and shared through LDS.
+template <int HD> struct GradLds {                 // byte offsets
+    static constexpr int K_AT = 0, Q_AT = K_AT + DC * (HD + 4) * 4, GT_AT = Q_AT + DC * (HD + 4) * 4, DG_AT = GT_AT + DC * SQ * 4;
+    static constexpr int DM_AT = DG_AT + DC * SQ * 4, ES_AT = DM_AT + DC * SQ * 4, F_AT = ES_AT + DC * SQ * 4;
+    static constexpr int BYTES = F_AT + (6 * DC + 4 * DC + 4 * 3 * DC + 8) * 4;
+};
+
+// What is left of the gradient, chunk by chunk in parallel, eight waves to a workgroup: a wave owns a quarter of the columns of
+// half of the rows of dQ and dK (a chunk's M and G are read twice, its other operands four times; with an eighth of the columns
+// and all rows it was 177 instead of 152 us at 672 chunks of f32, head dim 128; four waves 154).  The 64x64 matrices are formed tile by tile
+// and shared through LDS.
 template <int HD, typename T>
-__global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+__global__ __launch_bounds__(512) void delta_grad_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                                                          Rows rq, Rows rk, Rows rv, const T* __restrict__ DO,
                                                          const float* __restrict__ ALPHA, const float* __restrict__ BETA,
                                                          const float* __restrict__ US, const float* __restrict__ RS,
                                                          const float* __restrict__ MS, const float* __restrict__ GS,
                                                          T* __restrict__ DQ, T* __restrict__ DK, float* __restrict__ DALPHA,
                                                          float* __restrict__ DBETA, int L, int H, int NC) {
+    constexpr int CGS = 4, NR = 2, NN = HD / 64;   // column groups; row and column tiles of a wave
+    typedef GradLds<HD> S;
     extern __shared__ __align__(16) char lds[];
-    float(*ks)[HD + 4] = (float(*)[HD + 4])lds;
-    float(*qs)[HD + 4] = ks + DC;
-    float(*gt)[SQ] = (float(*)[SQ])(qs + DC);      // decays, [j][i]
-    float(*dg)[SQ] = gt + DC;                      // gradients of the decays, [j][i]
-    float(*dm)[SQ] = dg + DC;                      // dP o g, [i][j]
-    float(*es)[SQ] = dm + DC;                      // E + E^T
-    float* sa = (float*)(es + DC);
-    float* sb = sa + DC;
-    float* sg = sb + DC;
-    float(*sdb)[DC] = (float(*)[DC])(sg + DC);     // [jt][i]
-    float(*red)[3][DC] = (float(*)[3][DC])(sdb + 4);   // [wave][q.X, k.Y, k.Z][i]
-    float* srv = (float*)(red + 4);
-    float* fro = srv + DC;
-    float *sky = fro + 4, *sdg = sky + DC;         // k_i.Y_i, d(g_i)
-    constexpr int NN = HD / 64;                    // column tiles of a wave
+    float(*ks)[HD + 4] = (float(*)[HD + 4])(lds + S::K_AT);
+    float(*qs)[HD + 4] = (float(*)[HD + 4])(lds + S::Q_AT);
+    float(*gt)[SQ] = (float(*)[SQ])(lds + S::GT_AT);           // decays, [j][i]
+    float(*dg)[SQ] = (float(*)[SQ])(lds + S::DG_AT);           // gradients of the decays, [j][i]
+    float(*dm)[SQ] = (float(*)[SQ])(lds + S::DM_AT);           // dP o g, [i][j]
+    float(*es)[SQ] = (float(*)[SQ])(lds + S::ES_AT);           // E + E^T
+    float* sa = (float*)(lds + S::F_AT);
+    float *sb = sa + DC, *sg = sb + DC, *srv = sg + DC, *sky = srv + DC, *sdg = sky + DC;   // a, b, g, R.v, k.Y, d(g_i)
+    float(*sdb)[DC] = (float(*)[DC])(sdg + DC);                // [jt][i]
+    float(*red)[3][DC] = (float(*)[3][DC])(sdb + 4);           // [column group][q.X, k.Y, k.Z][i]
+    float* fro = (float*)(red + CGS);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g4 = (lane >> 4) * 4;
+    const int cg = wave % CGS, r0 = wave / CGS * NR, col = 16 * NN * cg + m;     // this wave's first column, its first row tile
     int64_t b;
     int h, c;
     chunk_place(blockIdx.x, H, NC, b, h, c);
     const int64_t ci = (b * H + h) * NC + c;
     const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
     const int64_t first = ((b * L + t0) * H + h) * HD, dense = (int64_t)H * HD;
-    rows_to_lds<HD, T>(chunk_of(K + rk.at(b, L, t0, h, HD), rk.ld, left), ks, tid);
-    rows_to_lds<HD, T>(chunk_of(Q + rq.at(b, L, t0, h, HD), rq.ld, left), qs, tid);
+    rows_to_lds<HD, T, 512>(chunk_of(K + rk.at(b, L, t0, h, HD), rk.ld, left), ks, tid);
+    rows_to_lds<HD, T, 512>(chunk_of(Q + rq.at(b, L, t0, h, HD), rq.ld, left), qs, tid);
     if (tid < DC) {
         const int64_t at = (b * L + t0 + tid) * H + h;
         sa[tid] = tid < left ? ALPHA[at] : 1.0f;
         sb[tid] = tid < left ? BETA[at] : 0.0f;
     }
-    (&sdb[0][0])[tid] = 0.f;
+    if (tid < 4 * DC) (&sdb[0][0])[tid] = 0.f;
     __syncthreads();
     if (wave == 0) chunk_decays(sa[lane], gt, lane);
     if (wave == 1) sg[lane] = chunk_prefix(sa[lane], lane);
@@ -818,18 +825,17 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
     const float* ub = US + ci * DC * HD;
     const float* rb = RS + ci * DC * HD;
     const ChunkOf<T> doc = chunk_of(DO + first, dense, left), vc = chunk_of(V + rv.at(b, L, t0, h, HD), rv.ld, left);
-    auto do4 = [&](int row, int col) -> f32x4_t { return widen4(doc.raw(row, col)); };
     // the 64x64 matrices: lane holds column i, rows j = 4g..4g+3 of a tile
-    for (int tile = wave; tile < TRI; tile += 4) {
+    for (int tile = wave; tile < TRI; tile += 8) {
         const int it = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, jt = tile - tri(it, 0);
         const int i = 16 * it + m, jr = 16 * jt + m;
         f32x4_t qk = {0.f, 0.f, 0.f, 0.f}, kk = qk, dp = qk, ru = qk;
 #pragma unroll
         for (int u = 0; u < HD / 16; ++u) {
-            const int col = 16 * u + g4;
-            const f32x4_t kj = *(const f32x4_t*)&ks[jr][col], qi = *(const f32x4_t*)&qs[i][col],
-                          ki = *(const f32x4_t*)&ks[i][col], uj = *(const f32x4_t*)(ub + jr * HD + col),
-                          ri = *(const f32x4_t*)(rb + i * HD + col), oi = do4(i, col);
+            const int at = 16 * u + g4;
+            const f32x4_t kj = *(const f32x4_t*)&ks[jr][at], qi = *(const f32x4_t*)&qs[i][at], ki = *(const f32x4_t*)&ks[i][at],
+                          uj = *(const f32x4_t*)(ub + jr * HD + at), ri = *(const f32x4_t*)(rb + i * HD + at),
+                          oi = widen4(doc.raw(i, at));
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 qk = mfma_f32(kj[r], qi[r], qk);
@@ -859,50 +865,52 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
         db += __shfl_xor(db, 32);
         if (lane < 16) sdb[jt][i] = db;
     }
-    // X, Y, Z and <G, M>
-    f32x4_t X[4][NN], Y[4][NN], Z[4][NN];
+    // X, Y, Z, <G, M> and R.v; two operand sets in turn
+    f32x4_t X[NR][NN], Y[NR][NN], Z[NR][NN];
 #pragma unroll
-    for (int it = 0; it < 4; ++it)
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int n = 0; n < NN; ++n) X[it][n] = Y[it][n] = Z[it][n] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-    const float* mb = MS + ci * HD * HD + wave * (HD / 4) + m;
-    const float* gb = GS + ci * HD * HD + wave * (HD / 4) + m;
+        for (int x = 0; x < NN; ++x) X[n][x] = Y[n][x] = Z[n][x] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    const float* mb = MS + ci * HD * HD + col;
+    const float* gb = GS + ci * HD * HD + col;
     float gm = 0.f, rdotv = 0.f;
     struct Operands {
-        f32x4_t o[4], r[4], u[4], rr, vv;
+        f32x4_t o[NR], r[NR], u[NR], rr, vv;
         float m[NN][4], g[NN][4];
     };
     auto load = [&](Operands& x, int u) {
-        const int col = 16 * u + g4;
+        const int at = 16 * u + g4;
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-            const int row = 16 * it + m;
-            x.o[it] = do4(row, col);
-            x.r[it] = *(const f32x4_t*)(rb + row * HD + col);
-            x.u[it] = *(const f32x4_t*)(ub + row * HD + col);
+        for (int n = 0; n < NR; ++n) {
+            const int row = 16 * (r0 + n) + m;
+            x.o[n] = widen4(doc.raw(row, at));
+            x.r[n] = *(const f32x4_t*)(rb + row * HD + at);
+            x.u[n] = *(const f32x4_t*)(ub + row * HD + at);
         }
 #pragma unroll
         for (int n = 0; n < NN; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                x.m[n][r] = mb[(col + r) * HD + 16 * n];
-                x.g[n][r] = gb[(col + r) * HD + 16 * n];
+                x.m[n][r] = mb[(at + r) * HD + 16 * n];
+                x.g[n][r] = gb[(at + r) * HD + 16 * n];
             }
-        x.rr = *(const f32x4_t*)(rb + (16 * wave + m) * HD + col);
-        x.vv = widen4(vc.raw(16 * wave + m, col));
+        if (wave < 4) {
+            x.rr = *(const f32x4_t*)(rb + (16 * wave + m) * HD + at);
+            x.vv = widen4(vc.raw(16 * wave + m, at));
+        }
     };
     auto use = [&](const Operands& x) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            rdotv = fmaf(x.rr[r], x.vv[r], rdotv);
+            if (wave < 4) rdotv = fmaf(x.rr[r], x.vv[r], rdotv);
 #pragma unroll
-            for (int n = 0; n < NN; ++n) {
-                gm = fmaf(x.m[n][r], x.g[n][r], gm);
+            for (int y = 0; y < NN; ++y) {
+                gm = fmaf(x.m[y][r], x.g[y][r], gm);
 #pragma unroll
-                for (int it = 0; it < 4; ++it) {
-                    X[it][n] = mfma_f32(x.o[it][r], x.m[n][r], X[it][n]);
-                    Y[it][n] = mfma_f32(x.r[it][r], x.m[n][r], Y[it][n]);
-                    Z[it][n] = mfma_f32(x.u[it][r], x.g[n][r], Z[it][n]);
+                for (int n = 0; n < NR; ++n) {
+                    X[n][y] = mfma_f32(x.o[n][r], x.m[y][r], X[n][y]);
+                    Y[n][y] = mfma_f32(x.r[n][r], x.m[y][r], Y[n][y]);
+                    Z[n][y] = mfma_f32(x.u[n][r], x.g[y][r], Z[n][y]);
                 }
             }
         }
@@ -918,23 +926,22 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) gm += __shfl_xor(gm, off);
-    if (lane == 0) fro[wave] = gm;
+    if (lane == 0) fro[wave] = r0 == 0 ? gm : 0.f;             // the other row half has the same columns
     rdotv += __shfl_xor(rdotv, 16);
     rdotv += __shfl_xor(rdotv, 32);
-    if (lane < 16) srv[16 * wave + m] = rdotv;
+    if (wave < 4 && lane < 16) srv[16 * wave + m] = rdotv;
 #pragma unroll
-    for (int it = 0; it < 4; ++it)
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int i = 16 * it + g4 + r;
+            const int i = 16 * (r0 + n) + g4 + r;
             float x = 0.f, y = 0.f, z = 0.f;
 #pragma unroll
-            for (int n = 0; n < NN; ++n) {
-                const int col = wave * (HD / 4) + 16 * n + m;
-                const float kv = ks[i][col];
-                x = fmaf(qs[i][col], X[it][n][r], x);
-                y = fmaf(kv, Y[it][n][r], y);
-                z = fmaf(kv, Z[it][n][r], z);
+            for (int w = 0; w < NN; ++w) {
+                const float kv = ks[i][col + 16 * w];
+                x = fmaf(qs[i][col + 16 * w], X[n][w][r], x);
+                y = fmaf(kv, Y[n][w][r], y);
+                z = fmaf(kv, Z[n][w][r], z);
             }
 #pragma unroll
             for (int off = 1; off < 16; off <<= 1) {
@@ -942,68 +949,72 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
                 y += __shfl_xor(y, off);
                 z += __shfl_xor(z, off);
             }
-            if (m == 0) red[wave][0][i] = x, red[wave][1][i] = y, red[wave][2][i] = z;
-            const float gi = sg[i], ge = gt[i][DC - 1], bgi = sb[i] * gi;
+            if (m == 0) red[cg][0][i] = x, red[cg][1][i] = y, red[cg][2][i] = z;
+            const float gi = sg[i];
 #pragma unroll
-            for (int n = 0; n < NN; ++n) {
-                Z[it][n][r] = ge * Z[it][n][r] - bgi * Y[it][n][r];
-                X[it][n][r] *= gi;
+            for (int w = 0; w < NN; ++w) {
+                Z[n][w][r] = gt[i][DC - 1] * Z[n][w][r] - sb[i] * gi * Y[n][w][r];
+                X[n][w][r] *= gi;
             }
         }
     __syncthreads();                               // dm, es, dg and the row sums are complete
     if (wave == 0) {                               // the last row of the decays carries k_j.Z_j and <G, M> too
-        sky[lane] = red[0][1][lane] + red[1][1][lane] + red[2][1][lane] + red[3][1][lane];
-        float d = red[0][0][lane] + red[1][0][lane] + red[2][0][lane] + red[3][0][lane] - sb[lane] * sky[lane];
-        if (lane == DC - 1) d += fro[0] + fro[1] + fro[2] + fro[3];
-        else dg[lane][DC - 1] += red[0][2][lane] + red[1][2][lane] + red[2][2][lane] + red[3][2][lane];
-        sdg[lane] = d;
+        float x = 0.f, y = 0.f, z = 0.f, f = 0.f;
+#pragma unroll
+        for (int n = 0; n < CGS; ++n) x += red[n][0][lane], y += red[n][1][lane], z += red[n][2][lane];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) f += fro[n];
+        sky[lane] = y;
+        sdg[lane] = x - sb[lane] * y + (lane == DC - 1 ? f : 0.f);
+        if (lane < DC - 1) dg[lane][DC - 1] += z;
     }
 #pragma unroll 1
     for (int jt = 0; jt < 4; ++jt) {
-        f32x4_t ad[4], ae[4];
-        float at[4][4], bk[NN][4], bq[NN][4];
+        f32x4_t ad[NR], ae[NR];
+        float at[NR][4], bk[NN][4], bq[NN][4];
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-            if (it >= jt) ad[it] = *(const f32x4_t*)&dm[16 * it + m][16 * jt + g4];
-            ae[it] = *(const f32x4_t*)&es[16 * it + m][16 * jt + g4];
+        for (int n = 0; n < NR; ++n) {
+            const int it = r0 + n;
+            ae[n] = *(const f32x4_t*)&es[16 * it + m][16 * jt + g4];
+            // dm holds the lower tiles only; the others' operands are zeros
+            const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+            ad[n] = it >= jt ? *(const f32x4_t*)&dm[16 * it + m][16 * jt + g4] : zero;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (it <= jt) at[it][r] = dm[16 * jt + g4 + r][16 * it + m];
+            for (int r = 0; r < 4; ++r) at[n][r] = it <= jt ? dm[16 * jt + g4 + r][16 * it + m] : 0.f;
         }
 #pragma unroll
-        for (int n = 0; n < NN; ++n)
+        for (int x = 0; x < NN; ++x)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int col = wave * (HD / 4) + 16 * n + m;
-                bk[n][r] = ks[16 * jt + g4 + r][col];
-                bq[n][r] = qs[16 * jt + g4 + r][col];
+                bk[x][r] = ks[16 * jt + g4 + r][col + 16 * x];
+                bq[x][r] = qs[16 * jt + g4 + r][col + 16 * x];
             }
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int n = 0; n < NN; ++n)
+            for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int it = 0; it < 4; ++it) {
-                    if (it >= jt) X[it][n] = mfma_f32(ad[it][r], bk[n][r], X[it][n]);
-                    if (it <= jt) Z[it][n] = mfma_f32(at[it][r], bq[n][r], Z[it][n]);
-                    Z[it][n] = mfma_f32(ae[it][r], bk[n][r], Z[it][n]);
+                for (int x = 0; x < NN; ++x) {
+                    X[n][x] = mfma_f32(ad[n][r], bk[x][r], X[n][x]);
+                    Z[n][x] = mfma_f32(at[n][r], bq[x][r], Z[n][x]);
+                    Z[n][x] = mfma_f32(ae[n][r], bk[x][r], Z[n][x]);
                 }
     }
     const ChunkOf<T> dqc = chunk_of((const T*)DQ + first, dense, left), dkc = chunk_of((const T*)DK + first, dense, left);
 #pragma unroll
-    for (int it = 0; it < 4; ++it)
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int n = 0; n < NN; ++n) {
-                const int i = 16 * it + g4 + r, col = wave * (HD / 4) + 16 * n + m;
-                dqc.put(i, col, X[it][n][r]);
-                dkc.put(i, col, Z[it][n][r]);
+            for (int x = 0; x < NN; ++x) {
+                const int i = 16 * (r0 + n) + g4 + r;
+                dqc.put(i, col + 16 * x, X[n][x][r]);
+                dkc.put(i, col + 16 * x, Z[n][x][r]);
             }
-    // da_t: D[t][i] = sum_{j < t} g_{t-1,j} d(g_ij) + g_{t-1} d(g_i), weighted with g_it and summed over i >= t.  A wave takes
-    // the row tile `wave` of t.
+    // da_t: D[t][i] = sum_{j < t} g_{t-1,j} d(g_ij) + g_{t-1} d(g_i), weighted with g_it and summed over i >= t.  The first four
+    // waves take a row tile of t each.
     __syncthreads();
-    {
+    if (wave < 4) {
         const int t = 16 * wave + m;
         float da[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -1036,9 +1047,8 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(const T* __restrict__ Q
             const int tt = 16 * wave + g4 + r;
             if (m == 0 && tt < left) DALPHA[(b * L + t0 + tt) * H + h] = da[r];
         }
-        if (lane < 16 && t < left) {
+        if (lane < 16 && t < left)
             DBETA[(b * L + t0 + t) * H + h] = sdb[0][t] + sdb[1][t] + sdb[2][t] + sdb[3][t] + srv[t] - sg[t] * sky[t];
-        }
     }
 }
 
@@ -1246,10 +1256,10 @@ int delta_bwd(const DeltaArgs& d, const void* d_out, const float* d_state, const
     }
     if (wide_scan<HD>(d)) VA_TRY((launch_rscan<HD, T, HD / 64>(d, w, d_out, d_state, dv, d_state_in, rs, gs, stream)));
     else VA_TRY((launch_rscan<HD, T, 1>(d, w, d_out, d_state, dv, d_state_in, rs, gs, stream)));
-    constexpr int lds = (2 * DC * (HD + 4) + 4 * DC * SQ + 3 * DC + 4 * DC + 12 * DC + DC + 4 + 2 * DC) * 4;
+    constexpr int lds = GradLds<HD>::BYTES;
     const auto fn = delta_grad_kernel<HD, T>;
     VA_TRY(reserve_lds("va_gated_delta_bwd", (const void*)fn, lds));
-    hipLaunchKernelGGL(fn, dim3((unsigned)n), dim3(256), lds, stream, (const T*)d.q, (const T*)d.k, (const T*)d.v, Rows{d.ldq},
+    hipLaunchKernelGGL(fn, dim3((unsigned)n), dim3(512), lds, stream, (const T*)d.q, (const T*)d.k, (const T*)d.v, Rows{d.ldq},
                        Rows{d.ldk}, Rows{d.ldv}, (const T*)d_out, d.alpha, d.beta, w.us, rs, w.ms, gs, (T*)dq, (T*)dk, dalpha, dbeta,
                        (int)d.L, (int)d.H, (int)d.chunks());
     VA_CHECK_LAUNCH("va_gated_delta_bwd (gradients)");
