@@ -285,3 +285,19 @@ def test_what_the_forward_keeps_equals_what_the_gradient_computes_again(B, L, H,
         assert torch.equal(x, y)
     with pytest.raises(ValueError):
         ops.gated_delta_bwd(out, s, *args, kept=kept[1:])
+
+
+@gpu
+def test_a_non_finite_token_stays_in_its_head_and_stream():
+    """It spreads over its chunk of 64 tokens and, through the state, over what follows; other heads and streams, and the
+    chunks before, give the bits they give without it."""
+    from vit_amd import ops
+    args = gpu_args(inputs(2, 200, 3, 64, torch.float32, True, seed="dn"))
+    out, s = ops.gated_delta_fwd(*args)
+    bad = [t.clone() for t in args]
+    bad[2][0, 130, 1, 5] = float("nan")
+    got, sg = ops.gated_delta_fwd(*bad)
+    assert torch.equal(got[1], out[1]) and torch.equal(sg[1], s[1])
+    assert torch.equal(got[0, :, [0, 2]], out[0, :, [0, 2]]) and torch.equal(sg[0, [0, 2]], s[0, [0, 2]])
+    assert torch.equal(got[0, :128, 1], out[0, :128, 1])
+    assert bool(torch.isnan(got[0, 130:, 1]).any()) and bool(torch.isnan(sg[0, 1]).any())
