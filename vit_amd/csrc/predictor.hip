@@ -59,8 +59,7 @@ __global__ __launch_bounds__(2 * HD) __attribute__((amdgpu_waves_per_eu(2))) voi
     const float* vb = V + (int64_t)b * L * row_stride + h * HD;
     const float* ab_src[2] = {ALPHA + (int64_t)b * L * H + h, BETA + (int64_t)b * L * H + h};
 
-    // the state as float pairs: the step arithmetic is written on pairs so that it maps to packed f32
-    // instructions on adjacent registers.  T[r][2j], T[r][2j+1] = row 2g + r, columns 16j + 4c .. + 3.
+    // the state as float pairs on adjacent registers.  T[r][2j], T[r][2j+1] = row 2g + r, columns 16j + 4c .. + 3.
     typedef __attribute__((ext_vector_type(2))) float f32x2_t;
     constexpr int NJ = HD / 16;
     const int cg = i & 3, row0 = (i >> 2) * 2;
