@@ -173,6 +173,15 @@ VA_DEVINL void stream_lengths(const AttnArgs& a, const Cache& c, int b, int& len
     nb = nb < 0 ? 0 : nb > a.n ? a.n : nb;
 }
 
+// Maximum over the four lane groups (lanes 16 and 32 apart): swapping rows of a register with its copy leaves one partner's
+// value in each, without the LDS round trip of a shuffle.
+VA_DEVINL float groups_max(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // Softmax weights of one 64-key tile for 16 queries and the rescaled running state.  s[kt] = raw scores of keys 16 kt + 4 g + r;
 // pf[u] = the tile's P^T operand for keys 32 u ..+31.  The running maximum is one of raw scores (the scale is positive), the
 // scale goes into the exponent's multiply-add.
@@ -186,8 +195,7 @@ VA_DEVINL float tile_softmax(f32x4_t (&s)[4], int key0, int g4, int limit, float
             if (MASK) s[kt][r] = key0 + 16 * kt + g4 + r < limit ? s[kt][r] : NEG_INF;
             top = fmaxf(top, s[kt][r]);
         }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = groups_max(top);
     const float now = fmaxf(mx, top);
     const float base = now == NEG_INF ? 0.f : now * scale2;     // nothing seen yet: every weight is exp2(-inf) = 0
     const float fade = __builtin_amdgcn_exp2f(fmaf(mx, scale2, -base));

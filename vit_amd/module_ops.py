@@ -267,9 +267,8 @@ class GatedLayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, o, gate, g, gamma, beta, eps):
         shape = o.shape
-        rows = [t.detach().reshape(-1, shape[-1]).contiguous() for t in (o, gate, g)]
-        gamma = gamma.detach()
-        y, mean, rstd = ops.gated_layernorm_fwd(*rows, gamma, beta.detach(), eps, keep=any(ctx.needs_input_grad))
+        rows = [t.reshape(-1, shape[-1]).contiguous() for t in (o, gate, g)]
+        y, mean, rstd = ops.gated_layernorm_fwd(*rows, gamma, beta, eps, keep=any(ctx.needs_input_grad))
         if mean is not None:
             ctx.save_for_backward(*rows, gamma, mean, rstd)
         return y.view(shape)
