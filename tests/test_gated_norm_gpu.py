@@ -126,6 +126,14 @@ def test_refusals():
     _, mean, rstd = ops.gated_layernorm_fwd(o, gate, g, gamma, beta)
     with pytest.raises(ValueError):
         ops.gated_layernorm_bwd(o, o, gate, g, gamma, mean[:4], rstd)
+    # no broadcasting between the three, and no gradient of the gradient
+    from vit_amd import module_ops
+    with pytest.raises(ValueError):
+        module_ops.gated_layernorm(o, gate[:1], g, gamma, beta)
+    x = o.clone().requires_grad_()
+    (first,) = torch.autograd.grad(module_ops.gated_layernorm(x, gate, g, gamma, beta).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        first.sum().backward()
 
 
 def test_refusals_without_a_gpu():

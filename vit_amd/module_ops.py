@@ -18,6 +18,7 @@ from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from ._lib import VitAmdError
@@ -243,6 +244,7 @@ class GatedDeltaFn(torch.autograd.Function):
         return out, new_state
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_out, d_state):
         q, k, v, alpha, beta, state, kept = ctx.saved_tensors
         if d_out is None and d_state is None:
@@ -274,6 +276,7 @@ class GatedLayerNormFn(torch.autograd.Function):
         return y.view(shape)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         rows, (gamma, mean, rstd) = ctx.saved_tensors[:3], ctx.saved_tensors[3:]
         shape = dy.shape
