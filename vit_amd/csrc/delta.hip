@@ -189,19 +189,55 @@ VA_DEVINL void rows_to_lds(const ChunkOf<T>& src, float (*dst)[HD + 4], int tid)
 }
 
 // ---------------------------------------------------------------------------------------------------------------
+// A chunk's rows in LDS as bf16 parts, plane n of a matrix at [n][row], rows of HD * 2 bytes in 16-byte pieces.  Columns
+// 32u + 16h + 4g + r of a row are element 4h + r of piece 4u + g, so one 16-byte read is a left operand's eight elements; the
+// pieces of row t stand at (piece ^ turn(t)), which spreads the sixteen rows of such a read, and the four rows times four
+// pieces of a transposed one, over all banks.
+template <int HD> VA_DEVINL int turn(int row) {
+    return HD == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+}
+template <int HD> VA_DEVINL int piece_at(int row, int piece) { return row * HD * 2 + ((piece ^ turn<HD>(row)) << 4); }
+// columns 4c .. 4c+3 of a row
+template <int HD> VA_DEVINL int quad_at(int row, int c) { return piece_at<HD>(row, (c >> 3) * 4 + (c & 3)) + ((c >> 2) & 1) * 8; }
+
+VA_DEVINL void put_rows(char* at, int plane, f32x4_t v) {        // f32: three parts
+    float x[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+        const u32x2_t w = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+        *(u32x2_t*)(at + n * plane) = w;
+        x[0] -= __uint_as_float(w[0] << 16);
+        x[1] -= __uint_as_float(w[0] & 0xffff0000u);
+        x[2] -= __uint_as_float(w[1] << 16);
+        x[3] -= __uint_as_float(w[1] & 0xffff0000u);
+    }
+}
+VA_DEVINL void put_rows(char* at, int, u32x2_t v) { *(u32x2_t*)at = v; }
+
+// left operand of rows 16 it.., columns 32u + 4g + {0..3, 16..19}
+template <int HD, int N>
+VA_DEVINL void row_frag(const char* x, int it, int u, int m, int g, bf16x8_t (&out)[N]) {
+    const char* at = x + piece_at<HD>(16 * it + m, 4 * u + g);
+#pragma unroll
+    for (int n = 0; n < N; ++n) out[n] = *(const bf16x8_t*)(at + n * DC * HD * 2);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
 // One workgroup of four waves per chunk.  K K^T and Q K^T tiles are formed transposed, D[j][i] = k_j.x_i, so that a lane holds
 // row i and four consecutive j; the wave with row tile w of K K^T (w + 1 tiles) takes row tile 3 - w of Q K^T, five tiles to
 // each.  Writes T and P; TRAIN: T^T and P^T as well, for the gradient's scan (P^T's tiles are formed the other way round).
 // Bound by memory when there are many chunks (100 KB of f32 rows and operands per chunk: 16 896 chunks of head dim 128 in
-// 470 us, 3.6 TB/s), by its chain of small systems when there are few (40 chunks: 12 us).  A and T lie over K in LDS so that
-// three workgroups share a CU.
+// 480 us, 3.5 TB/s), by its chain of small systems when there are few (40 chunks of bf16 rows: 9.9 us).  bf16 rows stay bf16
+// in LDS and are multiplied by the bf16 instruction, whose products of them are exact (with f32 copies and the f32 instruction
+// the 40 chunks took 12 us).  A and T lie over K in LDS so that three workgroups share a CU.
 template <int HD, typename T, bool TRAIN>
 __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q, const T* __restrict__ K, Rows rq, Rows rk,
                                                          const float* __restrict__ ALPHA, const float* __restrict__ BETA,
                                                          bf16_t* __restrict__ TF, bf16_t* __restrict__ PF, bf16_t* __restrict__ TT,
                                                          bf16_t* __restrict__ PT, float* __restrict__ GAM, int L, int H, int NC) {
     constexpr int NM = parts<T>::MID, NP = parts<T>::OUT;
-    constexpr int KBYTES = DC * (HD + 4) * 4, ABYTES = DC * SQ * 4 + DC * 20 * 4;
+    constexpr bool B16 = parts<T>::IN == 1;       // bf16 rows: the bf16 instruction multiplies them exactly
+    constexpr int KBYTES = B16 ? DC * HD * 2 : DC * (HD + 4) * 4, ABYTES = DC * SQ * 4 + DC * 20 * 4;
     __shared__ __align__(16) char lds[(KBYTES > ABYTES ? KBYTES : ABYTES)];
     __shared__ float gt[DC][SQ];
     __shared__ float sb[DC];
@@ -215,7 +251,16 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q
     const int64_t ci = (b * H + h) * NC + c;
     const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
     const ChunkOf<T> qc = chunk_of(Q + rq.at(b, L, t0, h, HD), rq.ld, left);
-    rows_to_lds<HD, T, 256>(chunk_of(K + rk.at(b, L, t0, h, HD), rk.ld, left), ks, tid);
+    const ChunkOf<T> kc = chunk_of(K + rk.at(b, L, t0, h, HD), rk.ld, left);
+    if constexpr (B16) {
+#pragma unroll
+        for (int p = 0; p < DC * HD / 4 / 256; ++p) {
+            const int idx = p * 256 + tid, row = idx / (HD / 4), c4 = idx % (HD / 4);
+            put_rows(lds + quad_at<HD>(row, c4), 0, kc.raw(row, c4 * 4));
+        }
+    } else {
+        rows_to_lds<HD, T, 256>(kc, ks, tid);
+    }
     const float mine = lane < left ? ALPHA[(b * L + t0 + lane) * H + h] : 1.0f;
     if (tid < DC) sb[tid] = tid < left ? BETA[(b * L + t0 + tid) * H + h] : 0.0f;
     if (wave == 0) chunk_decays(mine, gt, lane);
@@ -227,20 +272,41 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q
     // one copy of the code per wave: which tiles it forms is then known to the compiler
     auto tiles = [&](auto wv) {
         constexpr int WV = decltype(wv)::value, QT = 3 - WV;
+        if constexpr (B16) {
+            const int g = g4 >> 2;
+            auto q_frag = [&](int row, int u) {
+                const u32x2_t lo = qc.raw(row, 32 * u + g4), hi = qc.raw(row, 32 * u + g4 + 16);
+                return __builtin_bit_cast(bf16x8_t, (u32x4_t){lo[0], lo[1], hi[0], hi[1]});
+            };
 #pragma unroll
-        for (int u = 0; u < HD / 16; ++u) {
-            const int col = 16 * u + g4;
-            const f32x4_t mk = *(const f32x4_t*)&ks[16 * WV + m][col], mq = widen4(qc.raw(16 * QT + m, col));
+            for (int u = 0; u < HD / 32; ++u) {
+                bf16x8_t mk[1], kx[1];
+                row_frag<HD>(lds, WV, u, m, g, mk);
+                const bf16x8_t mq = q_frag(16 * QT + m, u);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                f32x4_t kx = {0.f, 0.f, 0.f, 0.f}, qx = kx;
-                if (x <= WV || x <= QT) kx = *(const f32x4_t*)&ks[16 * x + m][col];
-                if (TRAIN && x >= WV) qx = widen4(qc.raw(16 * x + m, col));
+                for (int x = 0; x < 4; ++x) {
+                    if (x <= WV || x <= QT) row_frag<HD>(lds, x, u, m, g, kx);
+                    if (x <= WV) kk[x] = mfma16(kx[0], mk[0], kk[x]);
+                    if (x <= QT) qk[x] = mfma16(kx[0], mq, qk[x]);
+                    if (TRAIN && x >= WV) pt[x] = mfma16(q_frag(16 * x + m, u), mk[0], pt[x]);
+                }
+            }
+        } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (x <= WV) kk[x] = mfma_f32(kx[r], mk[r], kk[x]);
-                    if (x <= QT) qk[x] = mfma_f32(kx[r], mq[r], qk[x]);
-                    if (TRAIN && x >= WV) pt[x] = mfma_f32(qx[r], mk[r], pt[x]);
+            for (int u = 0; u < HD / 16; ++u) {
+                const int col = 16 * u + g4;
+                const f32x4_t mk = *(const f32x4_t*)&ks[16 * WV + m][col], mq = widen4(qc.raw(16 * QT + m, col));
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    f32x4_t kx = {0.f, 0.f, 0.f, 0.f}, qx = kx;
+                    if (x <= WV || x <= QT) kx = *(const f32x4_t*)&ks[16 * x + m][col];
+                    if (TRAIN && x >= WV) qx = widen4(qc.raw(16 * x + m, col));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (x <= WV) kk[x] = mfma_f32(kx[r], mk[r], kk[x]);
+                        if (x <= QT) qk[x] = mfma_f32(kx[r], mq[r], qk[x]);
+                        if (TRAIN && x >= WV) pt[x] = mfma_f32(qx[r], mk[r], pt[x]);
+                    }
                 }
             }
         }
@@ -361,38 +427,6 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const T* __restrict__ Q
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// A chunk's rows in LDS as bf16 parts, plane n of a matrix at [n][row], rows of HD * 2 bytes in 16-byte pieces.  Columns
-// 32u + 16h + 4g + r of a row are element 4h + r of piece 4u + g, so one 16-byte read is a left operand's eight elements; the
-// pieces of row t stand at (piece ^ turn(t)), which spreads the sixteen rows of such a read, and the four rows times four
-// pieces of a transposed one, over all banks.
-template <int HD> VA_DEVINL int turn(int row) {
-    return HD == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
-}
-template <int HD> VA_DEVINL int piece_at(int row, int piece) { return row * HD * 2 + ((piece ^ turn<HD>(row)) << 4); }
-// columns 4c .. 4c+3 of a row
-template <int HD> VA_DEVINL int quad_at(int row, int c) { return piece_at<HD>(row, (c >> 3) * 4 + (c & 3)) + ((c >> 2) & 1) * 8; }
-
-VA_DEVINL void put_rows(char* at, int plane, f32x4_t v) {        // f32: three parts
-    float x[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-    for (int n = 0; n < 3; ++n) {
-        const u32x2_t w = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
-        *(u32x2_t*)(at + n * plane) = w;
-        x[0] -= __uint_as_float(w[0] << 16);
-        x[1] -= __uint_as_float(w[0] & 0xffff0000u);
-        x[2] -= __uint_as_float(w[1] << 16);
-        x[3] -= __uint_as_float(w[1] & 0xffff0000u);
-    }
-}
-VA_DEVINL void put_rows(char* at, int, u32x2_t v) { *(u32x2_t*)at = v; }
-
-// left operand of rows 16 it.., columns 32u + 4g + {0..3, 16..19}
-template <int HD, int N>
-VA_DEVINL void row_frag(const char* x, int it, int u, int m, int g, bf16x8_t (&out)[N]) {
-    const char* at = x + piece_at<HD>(16 * it + m, 4 * u + g);
-#pragma unroll
-    for (int n = 0; n < N; ++n) out[n] = *(const bf16x8_t*)(at + n * DC * HD * 2);
-}
 // left operand of the transposed rows: columns 16 ct.. of x, tokens 32u + 4g + {0..3, 16..19}
 template <int HD, int N>
 VA_DEVINL void col_frag(const char* x, int ct, int u, int lane, bf16x8_t (&out)[N]) {
