@@ -312,7 +312,8 @@ int va_gated_delta_seq(const float* q, const float* k, const float* v, const flo
  * q, k, v: rows of token (b, t) `ld*` elements apart (a multiple of 4, at least H*hd), heads side by side, all f32 or all
  * bf16 (is_bf16; 8-byte alignment is enough then); alpha, beta: contiguous f32 [B,L,H]; states f32 [B,H,hd,hd] (rows = value
  * index); out / gradients of q, k, v: contiguous [B,L,H,hd] of the inputs' type.  hd 64 or 128.  Products and states are
- * f32 whatever the type.  A non-finite token spreads over the 64-token chunk it lies in, earlier tokens included.
+ * f32 whatever the type.  A non-finite value reaches what it does in the recurrence (rows that meet one are
+ * formed again token by token); in the gradient it spreads over the 64-token chunk it lies in, earlier tokens included.
  *   fwd:  state_in NULL = zeros.  workspace: va_gated_delta_fwd_workspace_floats f32 values.  kept: NULL, or
  *         va_gated_delta_kept_floats f32 values that receive what the gradient needs besides the inputs.
  *   bwd:  d_out, and d_state (of the final state; NULL = zeros) -> dq, dk, dv, dalpha, dbeta [, d_state_in unless NULL];

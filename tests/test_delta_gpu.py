@@ -289,8 +289,8 @@ def test_what_the_forward_keeps_equals_what_the_gradient_computes_again(B, L, H,
 
 @gpu
 def test_a_non_finite_token_stays_in_its_head_and_stream():
-    """It spreads over its chunk of 64 tokens and, through the state, over what follows; other heads and streams, and the
-    chunks before, give the bits they give without it."""
+    """Through the state it spreads over what follows; other heads and streams, and the chunks before, give the bits they give
+    without it."""
     from vit_amd import ops
     args = gpu_args(inputs(2, 200, 3, 64, torch.float32, True, seed="dn"))
     out, s = ops.gated_delta_fwd(*args)
@@ -301,3 +301,33 @@ def test_a_non_finite_token_stays_in_its_head_and_stream():
     assert torch.equal(got[0, :, [0, 2]], out[0, :, [0, 2]]) and torch.equal(sg[0, [0, 2]], s[0, [0, 2]])
     assert torch.equal(got[0, :128, 1], out[0, :128, 1])
     assert bool(torch.isnan(got[0, 130:, 1]).any()) and bool(torch.isnan(sg[0, 1]).any())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,H,hd,state", [(2, 150, 2, 64, True), (1, 130, 3, 128, False), (65, 70, 2, 128, True)])
+def test_what_the_recurrence_leaves_finite_is_finite(B, L, H, hd, state, dtype):
+    """NaN and infinities in a value, a key, a query, both gates and the state: the same elements are non-finite as token by
+    token, and the others as close as ever."""
+    from vit_amd import ops
+    nan, inf = float("nan"), float("inf")
+    args = inputs(B, L, H, hd, dtype, state, seed="dx")
+    q, k, v, a, b, s = args
+    v[0, L - 20, 0, 5] = nan
+    v[B - 1, 10, 1, hd - 1] = -inf
+    k[0, 66, 1, 3] = nan
+    if B > 1:
+        q[1, 9, 0, 0] = inf
+        b[1, L - 3, 1] = nan
+    if B > 2:
+        a[2, 65, 0] = nan
+        k[3, 40, 1, 7] = inf
+        s[4, 1, 17, 2] = nan
+    want, want_s = recurrence(*(None if t is None else t.double() for t in args))
+    dev = gpu_args(args)
+    for keep in (False, True):
+        out, st = ops.gated_delta_fwd(*dev, keep=keep)[:2]
+        for name, got, ref in (("out", out, want), ("state", st, want_s)):
+            ok = torch.isfinite(ref)
+            assert torch.equal(torch.isfinite(got).cpu(), ok), name
+            close(torch.where(ok.cuda(), got, torch.zeros_like(got)), torch.where(ok, ref, torch.zeros_like(ref)), name)

@@ -143,3 +143,12 @@ def test_refusals_without_a_gpu():
         ops.gated_layernorm_fwd(*args)
     with pytest.raises(_lib.VitAmdError):
         ops.gated_layernorm_bwd(args[0], *args[:4], torch.zeros(4), torch.zeros(4))
+
+
+@pytest.mark.parametrize("M,D", [(0, 64), (1 << 26, 64), (1 << 24, 1028), (4, 66), (4, 4100)])
+def test_sizes_that_no_launch_can_take_are_refused(M, D):
+    """Before anything is launched: the addresses are never looked at."""
+    from vit_amd import _lib
+    lib = _lib.load()
+    assert lib.va_gated_layernorm_fwd(16, 16, 16, 0, 16, 16, 16, None, None, M, D, 1e-5, None) != 0
+    assert lib.va_gated_layernorm_bwd(*[16] * 4, 0, *[16] * 9, M, D, None) != 0

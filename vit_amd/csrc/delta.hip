@@ -541,6 +541,49 @@ VA_DEVINL void rows_times(const char* x, int u, const bf16x8_t (&b)[CG][NB], f32
     mfma_parts(a, b, acc, 0);
 }
 
+// The 16 CG rows of a head's state that a wave owns, and their outputs of the tokens from `from` on, token by token: 4 / CG lanes to a row, its elements in
+// registers.  The pointers stand at the head's first token; v, o and the states at the wave's first row.
+template <int HD, typename T, int CG>
+VA_DEVINL void rows_by_token(const T* q, const T* k, const T* v, int64_t ldq, int64_t ldk, int64_t ldv, const float* alpha,
+                             const float* beta, const float* s_in, T* o, float* s_out, int from, int L, int H, int lane) {
+    constexpr int ROWS = 16 * CG, N = HD * ROWS / 64 / 4;
+    const int row = lane % ROWS, col = lane / ROWS * 4 * N;
+    f32x4_t s[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[n] = s_in != nullptr ? *(const f32x4_t*)(s_in + row * HD + col + 4 * n) : (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    auto over_row = [](float x) {
+#pragma unroll
+        for (int off = ROWS; off < 64; off <<= 1) x += __shfl_xor(x, off);
+        return x;
+    };
+#pragma unroll 1
+    for (int t = 0; t < L; ++t) {
+        const ChunkOf<T> qt = chunk_of(q + t * ldq, ldq, 1), kt = chunk_of(k + t * ldk, ldk, 1);
+        const float a = alpha[(int64_t)t * H], b = beta[(int64_t)t * H];
+        float dot = 0.f, sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const f32x4_t x = widen4(kt.raw(0, col + 4 * n));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dot = fmaf(s[n][r], x[r], dot);
+        }
+        const float add = b * (chunk_of(v + t * ldv, ldv, 1).get(0, row) - a * over_row(dot));
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const f32x4_t x = widen4(kt.raw(0, col + 4 * n)), y = widen4(qt.raw(0, col + 4 * n));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[n][r] = fmaf(add, x[r], a * s[n][r]);
+                sum = fmaf(s[n][r], y[r], sum);
+            }
+        }
+        sum = over_row(sum);
+        if (lane < ROWS && t >= from) chunk_of(o + (int64_t)t * H * HD, (int64_t)H * HD, 1).put(0, row, sum);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) *(f32x4_t*)(s_out + row * HD + col + 4 * n) = s[n];
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // The sequential part.  A wave owns 16 CG columns (values of the head) of the state for the whole sequence: M in CG * HD/16
 // accumulator tiles; W waves share a chunk's K, Q, T and P through LDS, the next chunk's are requested while one computes.
@@ -548,11 +591,15 @@ VA_DEVINL void rows_times(const char* x, int u, const bf16x8_t (&b)[CG][NB], f32
 // Bound by its chain: per chunk and wave 360 matrix instructions (f32, head dim 128; 182 for bf16), about as many cycles of
 // vector work (splits, addresses) and of LDS reads, which one wave per SIMD runs one after the other: 7.7 us a chunk for f32, 5
 // for bf16; 512 heads x 2064 tokens of f32 in 0.8-0.95 ms (2.2 GB and 0.6 GB of operands).
+// A product with a zero does not silence a NaN, and an infinity has no parts: a token with either would reach earlier tokens of
+// its chunk.  A wave that ends with a non-finite output or state forms its rows again token by token, so that what the
+// recurrence leaves finite is finite; the outputs of the chunks before stay.
 template <int HD, typename T, int W, int CG, bool OUT, bool SAVE>
 __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
-                                                            Rows rq, Rows rk, Rows rv, const float* __restrict__ BETA,
-                                                            const bf16_t* __restrict__ TF, const bf16_t* __restrict__ PF,
-                                                            const float* __restrict__ GAM, const float* __restrict__ STATE_IN,
+                                                            Rows rq, Rows rk, Rows rv, const float* __restrict__ ALPHA,
+                                                            const float* __restrict__ BETA, const bf16_t* __restrict__ TF,
+                                                            const bf16_t* __restrict__ PF, const float* __restrict__ GAM,
+                                                            const float* __restrict__ STATE_IN,
                                                             T* __restrict__ O, float* __restrict__ STATE_OUT,
                                                             float* __restrict__ US, float* __restrict__ MS, int L, int H, int NC) {
     constexpr int NI = parts<T>::IN, NM = parts<T>::MID, NO = parts<T>::OUT;
@@ -579,6 +626,7 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
             M[x][u] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
             if (STATE_IN != nullptr) M[x][u] = *(const f32x4_t*)(STATE_IN + (bh * HD + v + 16 * x) * HD + 16 * u + g4);
         }
+    int bad = NC;                                 // first chunk with a non-finite output of this lane
     cr.request(0, NC);
     for (int c = 0; c < NC; ++c) {
         const int t0 = c * DC, left = L - t0 < DC ? L - t0 : DC;
@@ -659,12 +707,17 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
             blocks_times<4, false, NO>(pl, 0, 0, u0, o, lane);
             blocks_times<2, false, NO>(pl, 2, 1, u1, o, lane);
             const ChunkOf<T> oc = chunk_of((const T*)O + ((b * L + t0) * H + h) * HD, (int64_t)H * HD, left);
+            float seen = 0.f;                     // NaN with any output that is not finite
 #pragma unroll
             for (int x = 0; x < CG; ++x)
 #pragma unroll
                 for (int it = 0; it < 4; ++it)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) oc.put(16 * it + g4 + r, v + 16 * x, o[x][it][r]);
+                    for (int r = 0; r < 4; ++r) {
+                        oc.put(16 * it + g4 + r, v + 16 * x, o[x][it][r]);
+                        seen = fmaf(o[x][it][r], 0.f, seen);
+                    }
+            bad = seen != seen && c < bad ? c : bad;
         }
         const float gc = sg[DC - 1];
 #pragma unroll
@@ -678,7 +731,24 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
         }
         columns_times<HD, NI>(ks, f0, f1, M, lane);
     }
-    if (STATE_OUT != nullptr) {
+    if constexpr (OUT) {
+        float seen = 0.f;
+#pragma unroll
+        for (int x = 0; x < CG; ++x)
+#pragma unroll
+            for (int u = 0; u < HD / 16; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) seen = fmaf(M[x][u][r], 0.f, seen);
+        if (__any(bad < NC || seen != seen)) {
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) bad = min(bad, __shfl_xor(bad, off));
+            wait_vm0();                           // other lanes of the wave write over what this one has written
+            const int64_t first = b * L * H + h, row = bh * HD + v - m;
+            rows_by_token<HD, T, CG>(cr.q, cr.k, vb + v - m, rq.ld, rk.ld, rv.ld, ALPHA + first, cr.beta,
+                                     STATE_IN != nullptr ? STATE_IN + row * HD : nullptr, O + first * HD + v - m,
+                                     STATE_OUT + row * HD, bad * DC, L, H, lane);
+            return;
+        }
 #pragma unroll
         for (int x = 0; x < CG; ++x)
 #pragma unroll
@@ -1235,7 +1305,7 @@ int launch_scan(const DeltaArgs& d, const Work<T>& w, const float* state_in, voi
     const auto fn = delta_scan_kernel<HD, T, SCAN_W, CG, OUT, SAVE>;
     VA_TRY(reserve_lds("va_gated_delta", (const void*)fn, lds));
     hipLaunchKernelGGL(fn, dim3((unsigned)(d.B * d.H * (HD / 16 / (SCAN_W * CG)))), dim3(64 * SCAN_W), lds, stream, (const T*)d.q,
-                       (const T*)d.k, (const T*)d.v, Rows{d.ldq}, Rows{d.ldk}, Rows{d.ldv}, d.beta, w.tf, w.pf, w.gam, state_in,
+                       (const T*)d.k, (const T*)d.v, Rows{d.ldq}, Rows{d.ldk}, Rows{d.ldv}, d.alpha, d.beta, w.tf, w.pf, w.gam, state_in,
                        (T*)out, state_out, w.us, w.ms, (int)d.L, (int)d.H, (int)d.chunks());
     VA_CHECK_LAUNCH("va_gated_delta (scan)");
     return VA_OK;

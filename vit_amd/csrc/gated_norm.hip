@@ -223,7 +223,7 @@ int64_t gn_groups(int64_t M, int64_t D) {
 }
 
 int gn_check(const char* who, int64_t M, int64_t D, uintptr_t bits, int bf16) {
-    VA_CHECK_ARG(M > 0 && M < (1ll << 31), "%s: row count out of range", who);
+    VA_CHECK_ARG(M > 0 && M < (D <= 1024 ? 1ll << 26 : 1ll << 24), "%s: row count out of range", who);     // lanes of a grid: 2^32
     VA_CHECK_ARG(D > 0 && D % 4 == 0 && D <= 4096, "%s: width %lld not supported (a multiple of 4, at most 4096)", who, (long long)D);
     VA_CHECK_ARG(bits % (bf16 ? 8 : 16) == 0, "%s: misaligned operand", who);
     return VA_OK;
