@@ -331,3 +331,52 @@ def test_what_the_recurrence_leaves_finite_is_finite(B, L, H, hd, state, dtype):
             ok = torch.isfinite(ref)
             assert torch.equal(torch.isfinite(got).cpu(), ok), name
             close(torch.where(ok.cuda(), got, torch.zeros_like(got)), torch.where(ok, ref, torch.zeros_like(ref)), name)
+
+
+@gpu
+def test_a_state_changed_in_place_is_not_used_by_a_gradient():
+    from vit_amd import module_ops, ops
+    q, k, v, a, b, s = gpu_args(inputs(1, 5, 1, 64, torch.float32, True, seed="dv"))
+    v.requires_grad_()
+    out, _ = module_ops.gated_delta(q, k, v, a, b, s)
+    ops.gated_delta_step_(q[:, 0], k[:, 0], v.detach()[:, 0], a[:, 0], b[:, 0], s)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+
+
+def second_derivatives(f, args, directions):
+    """Gradients of sum(gradients of f * directions) in every input."""
+    leaves = [t.requires_grad_() for t in args]
+    out, s = f(*leaves)
+    first = torch.autograd.grad((out * directions[0]).sum() + (s * directions[1]).sum(), leaves, create_graph=True)
+    return torch.autograd.grad(sum((g * (i + 1)).pow(2).sum() for i, g in enumerate(first)), leaves)
+
+
+@gpu
+def test_second_derivatives_and_batched_gradients():
+    """They come from the formula in torch, f32: sums of a few hundred products within sums of a few hundred products, each good
+    to 1e-5 of its 2-norm; 1e-4 leaves room for both and for the tokens behind one another."""
+    from vit_amd import module_ops
+    args = inputs(2, 6, 2, 64, torch.float32, True, seed="d2")
+    go, gs = R.hashed_uniform("d2.go", (2, 6, 2, 64), 1.0), R.hashed_uniform("d2.gs", (2, 2, 64, 64), 0.5)
+    want = second_derivatives(recurrence, [t.double() for t in args], (go.double(), gs.double()))
+    got = second_derivatives(module_ops.gated_delta, gpu_args(args), (go.cuda(), gs.cuda()))
+    for g, w in zip(got, want):
+        assert (g.double().cpu() - w).norm() <= 1e-4 * w.norm()
+    # one tensor as two inputs
+    def twice(f, q, *rest):
+        out, s = f(q, q, *rest)
+        (first,) = torch.autograd.grad(out.pow(2).sum(), q, create_graph=True)
+        return torch.autograd.grad(first.pow(2).sum(), q)[0]
+    rest = [t.detach() for t in args[2:]]
+    want = twice(recurrence, args[0].detach().double().requires_grad_(), *(t.double() for t in rest))
+    got = twice(module_ops.gated_delta, args[0].detach().cuda().requires_grad_(), *gpu_args(rest))
+    assert (got.double().cpu() - want).norm() <= 1e-4 * want.norm()
+    # several gradients at once
+    dev = [t.detach().cuda().requires_grad_() for t in args]
+    out, _ = module_ops.gated_delta(*dev)
+    seeds = R.hashed_uniform("d2.seeds", (3, 2, 6, 2, 64), 1.0).cuda()
+    many = torch.autograd.grad(out, dev, seeds, is_grads_batched=True, retain_graph=True)
+    for i in range(3):
+        for a, b in zip(many, torch.autograd.grad(out, dev, seeds[i], retain_graph=True)):
+            assert (a[i] - b).norm() <= 1e-4 * b.norm()

@@ -123,3 +123,28 @@ def test_world_model_timestep_by_timestep():
     streams = model.new_predictor_streams(B, T, tokens.device)
     got = torch.cat([model.predict_stream(tokens[:, t * per:(t + 1) * per], streams) for t in range(T)], 1)
     assert got.shape == want.shape and rel(got, want) < REL_TOL + 2.0 ** -4
+    with pytest.raises(ValueError):
+        model.predict_stream(tokens[:, :per], streams[:2])
+    assert all(s.kv.lengths.tolist() == [T * per] * B for s in streams)
+
+
+def test_memory_layer_where_torch_must_see_every_operation():
+    """torch.func transforms, forward-mode derivatives, second derivatives, one state for all streams: what a layer of
+    torch operations allows."""
+    from vit_amd import surgical_world_model as swm
+    layer = filled(swm.GatedDeltaLayer(64, num_heads=2, head_dim=64), "mt").cuda()
+    x, t = (R.hashed_uniform(f"mt.{n}", (2, 9, 64), 1.0).cuda() for n in "xt")
+    s1 = R.hashed_uniform("mt.s", (1, 2, 64, 64), 0.2).cuda()
+    value = lambda y: layer(y)[0].pow(2).sum()                 # noqa: E731
+    leaf = x.clone().requires_grad_()
+    (want,) = torch.autograd.grad(value(leaf), leaf, create_graph=True)
+    assert rel(torch.func.grad(value)(x), want) < 1e-4
+    _, slope = torch.func.jvp(value, (x,), (t,))
+    assert abs(slope.item() - (want * t).sum().item()) <= 1e-4 * (want.norm() * t.norm()).item()
+    (second,) = torch.autograd.grad((want * t).sum(), leaf)
+    h = 1e-2
+    up, down = (torch.func.grad(value)(x + d * t) for d in (h, -h))
+    assert rel(second, (up - down) / (2 * h)) < 1e-2           # third derivatives times h^2, f32 noise over h
+    assert rel(layer(leaf, s1)[0], layer(leaf, s1.expand(2, 2, 64, 64).contiguous())[0]) == 0.0
+    with pytest.raises(ValueError):
+        layer(leaf[:0])

@@ -18,7 +18,6 @@ from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
 from ._lib import VitAmdError
@@ -230,6 +229,50 @@ class MlpFn(torch.autograd.Function):
         return dh, dw1, db1, dw2, db2, (g if ctx.has_resid else None), None
 
 
+_functorch_active = getattr(torch._C, "_are_functorch_transforms_active", lambda: False)
+
+
+def _addressless(*grads) -> bool:
+    """Gradients that come in batches (is_grads_batched=True, torch.func.vmap) have no memory of their own."""
+    for g in grads:
+        try:
+            if g is not None:
+                g.data_ptr()
+        except RuntimeError:
+            return True
+    return False
+
+
+def by_torch_alone() -> bool:
+    """True where every operation must be torch's own: torch.func transforms, forward-mode derivatives, autocast."""
+    return _functorch_active() or torch.autograd.forward_ad._current_level >= 0 or torch.is_autocast_enabled("cuda")
+
+
+def _torch_grads(formula, inputs, needed, grads):
+    """Gradients through a torch formulation: where they need a graph of their own (create_graph=True) or come in batches
+    (is_grads_batched=True), which the kernels do not give."""
+    graph = torch.is_grad_enabled()
+    with torch.enable_grad():
+        # an alias each: one tensor may be several of the inputs
+        alias = [None if x is None else x.view_as(x) if x.requires_grad else x for x in inputs]
+        pairs = [(y, g) for y, g in zip(formula(*alias), grads) if g is not None]
+        got = iter(torch.autograd.grad([y for y, _ in pairs], [x for x, need in zip(alias, needed) if need],
+                                       [g for _, g in pairs], create_graph=graph, allow_unused=True))
+    return tuple(next(got) if need else None for need in needed)
+
+
+def _delta_by_torch(q, k, v, alpha, beta, state):
+    dtype, (B, L, H, hd) = q.dtype, q.shape
+    q, k, v = (x.to(F32) for x in (q, k, v))
+    state = q.new_zeros(B, H, hd, hd) if state is None else state
+    outs = []
+    for t in range(L):
+        a, b, kt = alpha[:, t, :, None, None], beta[:, t, :, None, None], k[:, t, :, None, :]
+        state = a * (state - b * (state * kt).sum(-1, keepdim=True) * kt) + b * v[:, t, :, :, None] * kt
+        outs.append((state * q[:, t, :, None, :]).sum(-1))
+    return torch.stack(outs, 1).to(dtype), state
+
+
 class GatedDeltaFn(torch.autograd.Function):
     """Gated delta rule over a sequence (swm:523-555) with the gradients of every input and of the carried state."""
 
@@ -244,11 +287,12 @@ class GatedDeltaFn(torch.autograd.Function):
         return out, new_state
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_out, d_state):
         q, k, v, alpha, beta, state, kept = ctx.saved_tensors
         if d_out is None and d_state is None:
             return (None,) * 6
+        if torch.is_grad_enabled() or _addressless(d_out, d_state):
+            return _torch_grads(_delta_by_torch, (q, k, v, alpha, beta, state), ctx.needs_input_grad, (d_out, d_state))
         d_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if d_out is None else d_out.contiguous()
         want = state is not None and ctx.needs_input_grad[5]
         grads = ops.gated_delta_bwd(d_out, None if d_state is None else d_state.contiguous(), q, k, v, alpha, beta, state, want,
@@ -268,23 +312,30 @@ class GatedLayerNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, o, gate, g, gamma, beta, eps):
-        shape = o.shape
-        rows = [t.reshape(-1, shape[-1]).contiguous() for t in (o, gate, g)]
-        y, mean, rstd = ops.gated_layernorm_fwd(*rows, gamma, beta, eps, keep=any(ctx.needs_input_grad))
+        width = o.shape[-1]
+        y, mean, rstd = ops.gated_layernorm_fwd(*(t.reshape(-1, width) for t in (o, gate, g)), gamma, beta, eps,
+                                                keep=any(ctx.needs_input_grad))
         if mean is not None:
-            ctx.save_for_backward(*rows, gamma, mean, rstd)
-        return y.view(shape)
+            ctx.eps = eps
+            ctx.save_for_backward(o, gate, g, gamma, beta, mean, rstd)
+        return y.view(o.shape)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        rows, (gamma, mean, rstd) = ctx.saved_tensors[:3], ctx.saved_tensors[3:]
-        shape = dy.shape
-        grads = ops.gated_layernorm_bwd(dy.reshape(rows[0].shape).contiguous(), *rows, gamma, mean, rstd)
-        grads = [x.view(shape) for x in grads[:3]] + list(grads[3:])
+        o, gate, g, gamma, beta, mean, rstd = ctx.saved_tensors
+        if torch.is_grad_enabled() or _addressless(dy):
+            def formula(o, gate, g, gamma, beta):
+                x = o.to(F32) * gate.to(F32) * torch.nn.functional.silu(g.to(F32))
+                return (torch.nn.functional.layer_norm(x, x.shape[-1:], gamma, beta, ctx.eps).to(o.dtype),)
+            return _torch_grads(formula, (o, gate, g, gamma, beta), ctx.needs_input_grad[:5], (dy,)) + (None,)
+        width = o.shape[-1]
+        grads = ops.gated_layernorm_bwd(*(t.reshape(-1, width) for t in (dy.contiguous(), o, gate, g)), gamma, mean, rstd)
+        grads = [x.view(o.shape) for x in grads[:3]] + list(grads[3:])
         return tuple(x if need else None for x, need in zip(grads, ctx.needs_input_grad)) + (None,)
 
 
 def gated_layernorm(o, gate, g, gamma, beta, eps: float = 1e-5):
     """Differentiable `ops.gated_layernorm_fwd` over the last dimension; o, gate, g of one shape and type (f32 or bf16)."""
-    return GatedLayerNormFn.apply(o, gate, g, gamma, beta, float(eps))
+    if gate.shape != o.shape or g.shape != o.shape:
+        raise ValueError("gated_layernorm: o, gate and g must share one shape")
+    return GatedLayerNormFn.apply(o.contiguous(), gate.contiguous(), g.contiguous(), gamma, beta, float(eps))

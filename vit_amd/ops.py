@@ -418,7 +418,9 @@ class KVCache8:
     """Keys and values of `lengths` tokens per stream in 8 bits: e4m3 codes k8, v8 [B, H, capacity, hd] with one f32
     power-of-two scale per block of 64 tokens and head (k_scale, v_scale [B, H, capacity / 64]); the block that is not full yet
     lies in k_open, v_open [B, H, 64, hd] bf16.  A code times its scale is the value it stands for.  `max_len` is the host's
-    upper bound of the lengths (they live on the device): `kv8_append_` raises when it would pass the capacity."""
+    upper bound of the lengths (they live on the device): `kv8_append_` raises when it would pass the capacity.  A replayed
+    graph appends without the host: count its tokens into `max_len` yourself; on the device those that pass the capacity are
+    dropped."""
 
     def __init__(self, k8, v8, k_scale, v_scale, k_open, v_open, lengths, max_len: Optional[int] = None):
         if k8.dim() != 4 or k8.shape[2] % KV8_BLOCK or 0 in k8.shape:
@@ -659,6 +661,7 @@ def gated_delta_step_(q, k, v, alpha, beta, state):
     out = torch.empty(B, H, hd, dtype=q.dtype, device=q.device)
     check(_lib.load().va_gated_delta_step(_p(q), _p(k), _p(v), *lds, int(q.dtype == BF16), _p(alpha), _p(beta), _p(state),
                                           _p(out), B, H, hd, _stream()), "va_gated_delta_step")
+    torch.autograd.graph.increment_version(state)        # a graph that saved the state refuses to use it instead of being wrong
     return out
 
 

@@ -484,7 +484,8 @@ class GatedDeltaLayer(nn.Module):
             k = F.normalize(self.silu(self._causal_conv(self.k_conv1d, self.k_proj(x))), p=2, dim=-1)
             v = self.silu(self._causal_conv(self.v_conv1d, self.v_proj(x)))
             v, v_gate = v.chunk(2, dim=-1)
-            if x.is_cuda and q.dtype == torch.float32 and Dh in (64, 128):
+            if x.is_cuda and q.dtype == torch.float32 and Dh in (64, 128) and not module_ops.by_torch_alone():
+                state = None if state is None else state.expand(B, H, Dh, Dh)
                 with torch.cuda.device(x.device):
                     # the convolutions leave (batch, channel, time) order behind
                     out, new_state = module_ops.gated_delta(*(t.contiguous().view(B, L, H, Dh) for t in (q, k, v)), alpha, beta,
@@ -789,7 +790,9 @@ class SurgicalActionConditionedWorldModel(nn.Module):
         them -> the normalised predictor features of those tokens, as `forward` computes them for the whole sequence so
         far.  Each timestep costs its own tokens and one pass over the 8-bit cache instead of the whole sequence."""
         per_step = self.tokens_per_frame + 2
-        for blk, stream in zip(self.predictor_blocks, streams, strict=True):
+        if len(streams) != len(self.predictor_blocks):       # before any of them has taken the tokens
+            raise ValueError(f"predict_stream: {len(streams)} states for {len(self.predictor_blocks)} predictor blocks")
+        for blk, stream in zip(self.predictor_blocks, streams):
             tokens = blk.stream(tokens, stream, per_step)
         return self.predictor_norm(tokens)
 
