@@ -333,3 +333,33 @@ def test_refusals_without_a_gpu():
         ops.KVCache8.empty(1, 1, 64, 64, "cpu")
     with pytest.raises(ValueError):
         ops.KVCache8(torch.zeros(1, 1, 60, 64), *([None] * 6))
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [40, 130])
+def test_attention_of_more_streams_than_there_are_compute_units(n, hd):
+    """The other launch shape, with full and ragged row tiles; then a bad last token, which only the last query sees."""
+    from vit_amd import ops
+    B, H = 66, 4
+    lens = [n + 1 + (37 * b) % 90 for b in range(B)]
+    cache, k, v = filled(B, H, hd, lens, steps=(0.5, 1.0))
+    q = tokens(B, n, H, hd, "mu.q", 3.0)
+    out = ops.kv8_attn(q.cuda(), cache, tokens_per_timestep=1)
+    some = [0, 1, 33, B - 1]
+
+    class Some:
+        heads, lengths = H, cache.lengths[some]
+    for name in ("k8", "v8", "k_scale", "v_scale", "k_open", "v_open"):
+        t = getattr(cache, name)
+        setattr(Some, name, t.view(torch.uint8)[some].view(t.dtype) if t.dtype == torch.float8_e4m3fn else t[some])
+    close(out[some], *attention(q[some], Some, [n] * len(some), 1))
+    assert torch.isfinite(out).all()
+    dirty = ops.KVCache8.empty(B, H, hd, max(lens), "cuda")
+    for b, m in enumerate(lens):
+        v[b, m - 1, :, 3] = float("nan")
+    new = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ops.kv8_append_(dirty, k.cuda(), v.cuda(), new=new)
+    got = ops.kv8_attn(q.cuda(), dirty, tokens_per_timestep=1)
+    assert torch.equal(got[:, :-1, :, :3], out[:, :-1, :, :3]) and torch.equal(got[:, :-1, :, 4:], out[:, :-1, :, 4:])
+    assert torch.isfinite(got[:, :-1]).all() and torch.isnan(got[:, -1, :, 3]).all()

@@ -155,7 +155,7 @@ struct AttnArgs {
     const int32_t* new_;
     bf16_t* out;
     float *part_o, *part_ml;                 // [split][B * Hkv * rows][hd], [..][2]
-    int B, n, H, G, tpt, splits;
+    int B, n, H, G, tpt, splits, tile;       // tile: query rows of a workgroup
     float scale2;                            // softmax scale * log2(e)
 };
 
@@ -412,19 +412,22 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Cache c, AttnArgs a)
     }
 }
 
-// Many rows: bound by the matrix and vector pipes.  128 rows to a workgroup, 32 to a wave; a tile's keys and values are
-// widened to bf16 once and shared through LDS, double-buffered, with the tile after next already requested.  258 rows x 16
-// streams x 8 heads of 128 over up to 2064 tokens: 78-84 us, 330 TFLOP/s; bound by the length of a tile's chain (widening 22,
-// scores 13, values 10, the softmax between them) at four to eight waves per CU.
-template <int HD>
-__global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs a) {
+// Many rows: a tile's keys and values are widened to bf16 once and shared through LDS, double-buffered, with the tile after next
+// already requested; W waves with 16 CT rows each.  Bound by the length of a tile's chain (widening, scores, softmax, values)
+// where few waves share a SIMD, by the LDS reads of its operands where many do: 258 rows x 16 streams x 8 heads of 128 over
+// up to 2064 tokens in 67 us, 390 TFLOP/s, with nine waves of 16 rows to a workgroup and CU (four waves of 32 rows and a third
+// row tile of two rows: 78); 128 rows x 64 streams x 8 heads over 2064 tokens in 110 us with four waves of 32 rows, two
+// workgroups to a CU (twelve of 16: 122-143).
+template <int HD, int CT, int W>
+__global__ __launch_bounds__(64 * W, W == 12 ? 3 : 2) void kv8_attn_tile_kernel(Cache c, AttnArgs a) {
     constexpr int KSTR = HD * 2 + 16, VSTR = HD * 2 + 32, BUF = KB * (KSTR + VSTR);
-    constexpr int N = KB * HD / 16 / 256;    // 16-byte pieces of a tile per thread
+    constexpr int THREADS = 64 * W, PIECES = KB * HD / 16, N = (PIECES + THREADS - 1) / THREADS;    // 16 bytes of codes each
     extern __shared__ __align__(16) char lds[];
     __shared__ int sbad[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4, g4 = g * 4;
     const int rows = a.n * a.G, h = blockIdx.y, b = blockIdx.z;
-    const int split = blockIdx.x % a.splits, row0 = (int)(blockIdx.x / a.splits) * 128 + wave * 32;
+    const int split = blockIdx.x % a.splits, first_row = (int)(blockIdx.x / a.splits) * a.tile, end_row = min(first_row + a.tile, rows);
+    const int row0 = first_row + wave * 16 * CT;
     int len, nb;
     stream_lengths(a, c, b, len, nb);
     const int64_t bh = (int64_t)b * a.H + h;
@@ -432,25 +435,24 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
     const float *ksp = c.ks + bh * (c.cap / KB), *vsp = c.vs + bh * (c.cap / KB);
     const int full = len / KB;
     // the workgroup's last visible key: limits do not fall with the row
-    const int first_row = (int)(blockIdx.x / a.splits) * 128, last_row = min(first_row + 127, rows - 1);
-    const int last_q = min(last_row / a.G, nb - 1);
+    const int last_row = end_row - 1, last_q = min(last_row / a.G, nb - 1);
     const int most = last_q >= first_row / a.G ? key_limit(a, last_q, len, nb) : 0;
     // keys that every row of the workgroup sees
     const int all_see = last_row / a.G < nb ? key_limit(a, first_row / a.G, len, nb) : 0;
-    const bool idle = row0 >= rows;          // a wave without rows only helps to load
+    const bool idle = row0 >= end_row;          // a wave without rows only helps to load
     const int tiles = (most + KB - 1) / KB;
     const int per = (tiles + a.splits - 1) / a.splits, t_begin = split * per, t_end = min(tiles, t_begin + per);
-    bf16x8_t qf[2][HD / 32];
-    int limit[2], least = 0x7fffffff;
+    bf16x8_t qf[CT][HD / 32];
+    int limit[CT], least = 0x7fffffff;
 #pragma unroll
-    for (int ct = 0; ct < 2; ++ct) {
+    for (int ct = 0; ct < CT; ++ct) {
         const int row = row0 + 16 * ct + m;
-        limit[ct] = row < rows ? key_limit(a, row / a.G, len, nb) : 0;
-        if (row < rows) least = min(least, limit[ct]);
+        limit[ct] = row < end_row ? key_limit(a, row / a.G, len, nb) : 0;
+        if (row < end_row) least = min(least, limit[ct]);
 #pragma unroll
         for (int f = 0; f < HD / 32; ++f) {
             u32x4_t v = {0u, 0u, 0u, 0u};
-            if (row < rows)
+            if (row < end_row)
                 v = *(const u32x4_t*)(a.q + b * a.bsq + (int64_t)(row / a.G) * a.ldq + ((int64_t)h * a.G + row % a.G) * HD + 32 * f + 8 * g);
             qf[ct][f] = as_frag(v);
         }
@@ -458,12 +460,14 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) least = min(least, __shfl_xor(least, off));
     least = __builtin_amdgcn_readfirstlane(least);
-    f32x4_t o[2][HD / 16];
-    float mx[2] = {NEG_INF, NEG_INF}, sum[2] = {0.f, 0.f};
+    f32x4_t o[CT][HD / 16];
+    float mx[CT], sum[CT];
 #pragma unroll
-    for (int ct = 0; ct < 2; ++ct)
+    for (int ct = 0; ct < CT; ++ct) {
+        mx[ct] = NEG_INF, sum[ct] = 0.f;
 #pragma unroll
         for (int ht = 0; ht < HD / 16; ++ht) o[ct][ht] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    }
     u32x4_t kr[N], vr[N];
     float kscale = 1.f, vscale = 1.f;
     auto request = [&](int t) {
@@ -471,8 +475,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
         const int64_t at = (int64_t)t * KB * HD;
 #pragma unroll
         for (int p = 0; p < N; ++p) {
-            kr[p] = span16(kb + at, KB * HD, (p * 256 + tid) * 16);
-            vr[p] = span16(vb + at, KB * HD, (p * 256 + tid) * 16);
+            kr[p] = span16(kb + at, KB * HD, (p * THREADS + tid) * 16);      // zeros for threads without a piece
+            vr[p] = span16(vb + at, KB * HD, (p * THREADS + tid) * 16);
         }
         kscale = ksp[t];
         vscale = vsp[t];
@@ -486,11 +490,12 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
         int id = tid;
         asm volatile("" : "+v"(id));
         if (t < full) {
-            constexpr int C = HD / 16, ROWS = 256 / C;      // pieces of a row, rows of a pass
+            constexpr int C = HD / 16, ROWS = THREADS / C;  // pieces of a row, rows of a pass
             char* kt_ = lds + (t & 1) * BUF + (id / C) * KSTR + (id % C) * 32;
             char* vt_ = lds + (t & 1) * BUF + KB * KSTR + (id / C) * VSTR + (id % C) * 32;
 #pragma unroll
             for (int p = 0; p < N; ++p) {
+                if (PIECES % THREADS != 0 && p * W + wave >= PIECES / 64) continue;
                 *(u32x4_t*)(kt_ + p * ROWS * KSTR) = widen8(kr[p][0], kr[p][1], kscale);
                 *(u32x4_t*)(kt_ + p * ROWS * KSTR + 16) = widen8(kr[p][2], kr[p][3], kscale);
                 const u32x4_t lo = widen8(vr[p][0], vr[p][1], vscale), hi = widen8(vr[p][2], vr[p][3], vscale);
@@ -499,14 +504,15 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
                 *(u32x4_t*)(vt_ + p * ROWS * VSTR + 16) = hi;
             }
         } else {
-            constexpr int C = HD / 8, ROWS = 256 / C;
+            constexpr int C = HD / 8, ROWS = THREADS / C;
             const int left = len - t * KB;
             char* kt_ = lds + (t & 1) * BUF + (id / C) * KSTR + (id % C) * 16;
             char* vt_ = lds + (t & 1) * BUF + KB * KSTR + (id / C) * VSTR + (id % C) * 16;
 #pragma unroll
-            for (int p = 0; p < 2 * N; ++p) {
-                const u32x4_t k = span16(c.ko + bh * KB * HD, left * HD * 2, (p * 256 + id) * 16);
-                const u32x4_t v = span16(c.vo + bh * KB * HD, left * HD * 2, (p * 256 + id) * 16);
+            for (int p = 0; p < (2 * PIECES + THREADS - 1) / THREADS; ++p) {
+                if (2 * PIECES % THREADS != 0 && p * W + wave >= 2 * PIECES / 64) continue;
+                const u32x4_t k = span16(c.ko + bh * KB * HD, left * HD * 2, (p * THREADS + id) * 16);
+                const u32x4_t v = span16(c.vo + bh * KB * HD, left * HD * 2, (p * THREADS + id) * 16);
                 bad |= any_nonfinite(v);
                 *(u32x4_t*)(kt_ + p * ROWS * KSTR) = k;
                 *(u32x4_t*)(vt_ + p * ROWS * VSTR) = v;
@@ -528,21 +534,21 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
         int ln = lane;                       // as in place(): addresses are formed anew instead of kept and spilled
         asm volatile("" : "+v"(ln));
         const char *kt_ = lds + (t & 1) * BUF, *vt_ = kt_ + KB * KSTR;
-        f32x4_t s[2][4];
+        f32x4_t s[CT][4];
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
-            s[0][kt] = s[1][kt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            s[0][kt] = s[CT - 1][kt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int f = 0; f < HD / 32; ++f) {
                 const bf16x8_t kf = as_frag(*(const u32x4_t*)(kt_ + (ln & 15) * KSTR + (ln >> 4) * 16 + 16 * kt * KSTR + 64 * f));
                 s[0][kt] = mfma16(kf, qf[0][f], s[0][kt]);
-                s[1][kt] = mfma16(kf, qf[1][f], s[1][kt]);
+                if (CT > 1) s[CT - 1][kt] = mfma16(kf, qf[CT - 1][f], s[CT - 1][kt]);
             }
         }
         const bool edge = (t + 1) * KB > least;
-        bf16x8_t pf[2][2];
+        bf16x8_t pf[CT][2];
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
+        for (int ct = 0; ct < CT; ++ct) {
             const float fade = edge ? tile_softmax<true>(s[ct], t * KB, g4, limit[ct], a.scale2, mx[ct], sum[ct], pf[ct])
                                     : tile_softmax<false>(s[ct], t * KB, g4, limit[ct], a.scale2, mx[ct], sum[ct], pf[ct]);
 #pragma unroll
@@ -550,24 +556,24 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(Cache c, AttnArgs
         }
         if (edge && flagged) {
             tile_pv<HD>(vt_, VSTR, pf[0], o[0], ln, true, limit[0] - t * KB);
-            tile_pv<HD>(vt_, VSTR, pf[1], o[1], ln, true, limit[1] - t * KB);
+            if (CT > 1) tile_pv<HD>(vt_, VSTR, pf[CT - 1], o[CT - 1], ln, true, limit[CT - 1] - t * KB);
         } else {
 #pragma unroll
             for (int ht = 0; ht < HD / 16; ++ht)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const bf16x8_t vf = v_frag(vt_, VSTR, ht, u, ln);
-                    o[0][ht] = mfma16(vf, pf[0][u], o[0][ht]);
-                    o[1][ht] = mfma16(vf, pf[1][u], o[1][ht]);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) o[ct][ht] = mfma16(vf, pf[ct][u], o[ct][ht]);
                 }
         }
     }
 #pragma unroll
-    for (int ct = 0; ct < 2; ++ct) {
+    for (int ct = 0; ct < CT; ++ct) {
         sum[ct] += __shfl_xor(sum[ct], 16);
         sum[ct] += __shfl_xor(sum[ct], 32);
         const int row = row0 + 16 * ct + m;
-        if (row >= rows) continue;
+        if (row >= end_row) continue;
         if (a.splits == 1) {
             const float inv = sum[ct] == 0.f ? 0.f : 1.f / sum[ct];                     // nothing seen: zeros
             bf16_t* dst = a.out + (((int64_t)b * a.n + row / a.G) * a.H * a.G + (int64_t)h * a.G + row % a.G) * HD + g4;
@@ -612,13 +618,22 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a) {
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------
+// Query rows of a workgroup where there are many (a multiple of 16).  While that makes no more workgroups than CUs, up to twelve
+// waves of 16 rows, the rows spread evenly over the workgroups (128 rows x 32 streams x 8 heads over 2064 tokens: 68 us, as
+// below 76; 192 x 16 x 8: 56, 78).  From there on four waves of 32 rows, which read each key from LDS half as often and let a
+// second workgroup onto the CU (128 rows x 48 streams x 8 heads: 97 us, as above 121).
+int64_t kv8_even_tiles(int64_t rows) { return (rows + 191) / 192; }
+bool kv8_spread(int64_t B, int64_t H, int64_t rows) { return B * H * kv8_even_tiles(rows) <= 256; }
+int kv8_tile(int64_t B, int64_t H, int64_t rows) {
+    const int64_t units = (rows + 15) / 16, tiles = kv8_even_tiles(rows);
+    return kv8_spread(B, H, rows) ? (int)((units + tiles - 1) / tiles) * 16 : 128;
+}
 // Pieces that the keys are split into.  Few rows: two workgroups to a CU where there are not as many (streams, heads); many rows:
-// one (256 row tiles in two pieces each were 87 us with their join, whole 79); never a piece below four tiles per wave (few
-// rows) or per workgroup (many rows).  `max_len` only steers this.
+// at most one; never a piece below four tiles per wave (few rows) or per workgroup (many rows).  `max_len` only steers this.
 int kv8_splits(int64_t B, int64_t H, int64_t rows, int64_t max_len) {
-    const int64_t groups = B * H * (rows <= 16 ? 1 : (rows + 127) / 128), tiles = (max_len + KB - 1) / KB;
-    const int64_t want = rows <= 16 ? 2 * 256 : 256;
-    int64_t s = (want + groups - 1) / groups;
+    const int64_t tile = rows <= 16 ? 16 : kv8_tile(B, H, rows);
+    const int64_t groups = B * H * ((rows + tile - 1) / tile), tiles = (max_len + KB - 1) / KB;
+    int64_t s = rows <= 16 ? (2 * 256 + groups - 1) / groups : 256 / groups;
     const int64_t most = rows <= 16 ? (tiles + 15) / 16 : (tiles + 3) / 4;
     s = s < most ? s : most;
     return (int)(s < 1 ? 1 : s > 128 ? 128 : s);
@@ -640,13 +655,14 @@ int kv8_attn(const Cache& c, const AttnArgs& a, hipStream_t stream) {
         hipLaunchKernelGGL(kv8_attn_rows_kernel<HD>, dim3(a.splits, a.H, a.B), dim3(256), 0, stream, c, a);
     } else {
         constexpr int lds = 2 * KB * (HD * 4 + 48);
-        if (hipFuncSetAttribute((const void*)kv8_attn_tile_kernel<HD>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+        const bool spread = kv8_spread(a.B, a.H, rows);
+        const auto fn = spread ? kv8_attn_tile_kernel<HD, 1, 12> : kv8_attn_tile_kernel<HD, 2, 4>;
+        if (hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
             (void)hipGetLastError();
             va_set_error("va_kv8_attn: cannot reserve %d bytes of LDS", lds);
             return VA_ERR_LAUNCH;
         }
-        hipLaunchKernelGGL(kv8_attn_tile_kernel<HD>, dim3((unsigned)((rows + 127) / 128 * a.splits), a.H, a.B), dim3(256), lds, stream,
-                           c, a);
+        hipLaunchKernelGGL(fn, dim3((unsigned)((rows + a.tile - 1) / a.tile * a.splits), a.H, a.B), dim3(spread ? 768 : 256), lds, stream, c, a);
     }
     VA_CHECK_LAUNCH("va_kv8_attn");
     if (a.splits > 1) {
@@ -708,7 +724,7 @@ extern "C" int va_kv8_attn(const void* q, int64_t ldq, int64_t bsq, const int32_
     VA_CHECK_ARG(splits == 1 || workspace, "va_kv8_attn: null workspace");
     const Cache c = {(const uint8_t*)k8, (const uint8_t*)v8, k_scale, v_scale, (const bf16_t*)k_open, (const bf16_t*)v_open, lengths, cap};
     AttnArgs a = {(const bf16_t*)q, ldq, bsq, new_tokens, (bf16_t*)out, workspace, nullptr, (int)B, (int)n, (int)H, (int)group,
-                  (int)tokens_per_timestep, splits, scale * LOG2E};
+                  (int)tokens_per_timestep, splits, kv8_tile(B, H, n * group), scale * LOG2E};
     if (splits > 1) a.part_ml = workspace + (int64_t)splits * B * H * n * group * hd;
     return hd == 128 ? kv8_attn<128>(c, a, stream) : kv8_attn<64>(c, a, stream);
 }
