@@ -32,7 +32,7 @@ struct Cache {
 // ---- append ---------------------------------------------------------------------------------------------------
 // One workgroup per block that the call touches, head and stream, keys or values.  Where the open block fills up and a
 // later one is left open, one workgroup does both: it has read the open block before it writes the new one over it.  Bound by
-// launches for single tokens (4 us), by memory for long calls (16 streams x 1290 tokens x 8 heads of 128: 23 us, 5.5 TB/s).
+// launches for single tokens (below 4 us), by memory for long calls (16 streams x 1290 tokens x 8 heads of 128: 23 us, 5.5 TB/s).
 template <int HD>
 __global__ __launch_bounds__(256) void kv8_append_kernel(const bf16_t* __restrict__ K, const bf16_t* __restrict__ V, int64_t ldk,
                                                          int64_t ldv, int64_t bsk, int64_t bsv, const int32_t* __restrict__ NEW,
@@ -56,22 +56,20 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(const bf16_t* __restric
     const bf16_t* src = (val ? V + b * bsv : K + b * bsk) + h * HD;
     const int64_t ld = val ? ldv : ldk;
     bf16_t* open = (val ? VO : KO) + bh * KB * HD;
-    u32x4_t x[N];
-    uint32_t big = 0;
+    if (whole) {                             // (a block that stays open is not read)
+        u32x4_t x[N];
+        uint32_t big = 0;
 #pragma unroll
-    for (int p = 0; p < N; ++p) {
-        const int idx = p * 256 + tid, row = idx / (HD / 8), c = (idx % (HD / 8)) * 8;
-        const int64_t t = start + row;
-        x[p] = (u32x4_t){0u, 0u, 0u, 0u};
-        if (t < len) x[p] = *(const u32x4_t*)(open + row * HD + c);
-        else if (t < total) x[p] = *(const u32x4_t*)(src + (t - len) * ld + c);
+        for (int p = 0; p < N; ++p) {
+            const int idx = p * 256 + tid, row = idx / (HD / 8), c = (idx % (HD / 8)) * 8;
+            const int64_t t = start + row;
+            x[p] = t < len ? *(const u32x4_t*)(open + row * HD + c) : *(const u32x4_t*)(src + (t - len) * ld + c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {        // magnitudes of finite bf16 numbers order like their bits
-            const uint32_t lo = x[p][e] & 0x7fffu, hi = (x[p][e] >> 16) & 0x7fffu;
-            big = max(big, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+            for (int e = 0; e < 4; ++e) {    // magnitudes of finite bf16 numbers order like their bits
+                const uint32_t lo = x[p][e] & 0x7fffu, hi = (x[p][e] >> 16) & 0x7fffu;
+                big = max(big, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+            }
         }
-    }
-    if (whole) {
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, off));
         if ((tid & 63) == 0) wmax[tid >> 6] = big;
