@@ -345,7 +345,8 @@ int va_gated_delta_step(const void* q, const void* k, const void* v, int64_t ldq
  *   attn:   q bf16 [B,n,H*group,hd] strided like k; out bf16 contiguous.  The queries are the newest n (new_tokens[b]) tokens
  *           of each stream, already appended: query i stands at p = lengths[b] - new_tokens[b] + i and sees all held tokens
  *           (tokens_per_timestep 0) or those before the end of its timestep, j < (p / T + 1) T (T = 1: causal).  Rows from
- *           new_tokens[b] on, and queries that see nothing, are zeros.  Query head h reads key/value head h / group.
+ *           new_tokens[b] on, and queries that see nothing, are zeros; a NaN in a query or in what it sees reaches its result.
+ *           Query head h reads key/value head h / group.
  *           scale must be positive.  max_len (<= cap): an upper bound of the lengths if the host has one; it only chooses how many pieces the keys are
  *           split into.  workspace: va_kv8_attn_workspace_floats f32 values for the same sizes (may be 0). */
 int va_kv8_append(const void* k, const void* v, int64_t ldk, int64_t ldv, int64_t bsk, int64_t bsv, const int32_t* new_tokens,

@@ -1,0 +1,89 @@
+"""GPU: attention over the 8-bit cache where it can go wrong without a wrong answer showing in ordinary inputs: NaN that
+queries do see, whatever the launch shape."""
+import pytest
+import torch
+
+from oracle import ref_cpu as R
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def tokens(B, n, H, hd, name, scale=2.0):
+    return R.hashed_uniform(name, (B, n, H, hd), scale).to(BF16)
+
+
+def cache_of(k, v, capacity=None):
+    from vit_amd import ops
+    cache = ops.KVCache8.empty(k.shape[0], k.shape[2], k.shape[3], capacity or k.shape[1], "cuda")
+    return ops.kv8_append_(cache, k.cuda(), v.cuda())
+
+
+# (tokens held, queries): few rows in one piece and in several, many rows in one piece (both tile shapes) and in several
+SHAPES = [(200, 1), (2900, 1), (2900, 16), (200, 64), (200, 150), (2900, 64), (2900, 150)]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("total,n", SHAPES)
+def test_a_nan_query_gives_nan_and_no_other_row_changes(total, n, hd):
+    from vit_amd import ops
+    B, H = 2, 2
+    cache = cache_of(tokens(B, total, H, hd, "e.k"), tokens(B, total, H, hd, "e.v"))
+    q = tokens(B, n, H, hd, "e.q").cuda()
+    clean = ops.kv8_attn(q, cache, tokens_per_timestep=1)
+    assert torch.isfinite(clean).all()
+    q[1, n - 1, 0, 5] = float("nan")
+    got = ops.kv8_attn(q, cache, tokens_per_timestep=1)
+    assert torch.isnan(got[1, n - 1, 0]).all()
+    got[1, n - 1, 0] = clean[1, n - 1, 0]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("total,n", SHAPES)
+def test_a_block_of_nan_keys_reaches_every_query_that_sees_it(total, n, hd):
+    """A wave or a piece of the keys may hold nothing but such a block; its place makes it the first, a middle or the last
+    one of the tokens."""
+    from vit_amd import ops
+    B, H = 1, 2
+    k, v, q = tokens(B, total, H, hd, "b.k"), tokens(B, total, H, hd, "b.v"), tokens(B, n, H, hd, "b.q").cuda()
+    clean = ops.kv8_attn(q, cache_of(k, v), tokens_per_timestep=1)
+    for block in sorted({0, 1, total // 64 - 1}):
+        bad = k.clone()
+        bad[:, 64 * block:64 * block + 64, 1] = float("nan")
+        got = ops.kv8_attn(q, cache_of(bad, v), tokens_per_timestep=1)
+        sees = total - n + torch.arange(n) >= 64 * block
+        assert torch.isnan(got[0, sees, 1]).all(), block
+        assert torch.equal(got[0, ~sees, 1], clean[0, ~sees, 1]) and torch.equal(got[:, :, 0], clean[:, :, 0]), block
+
+
+@pytest.mark.parametrize("n", [1, 17, 140])
+def test_a_stream_of_one_nan_token_beside_streams_without_tokens(n):
+    from vit_amd import ops
+    hd = 64
+    k, v, q = tokens(3, n, 1, hd, "o.k"), tokens(3, n, 1, hd, "o.v"), tokens(3, n, 1, hd, "o.q").cuda()
+    k[1, 0] = float("nan")
+    cache = ops.KVCache8.empty(3, 1, hd, 4096, "cuda")
+    new = torch.tensor([0, 1, n], dtype=torch.int32, device="cuda")
+    ops.kv8_append_(cache, k.cuda(), v.cuda(), new=new)
+    for bound in (n, 4096):                                   # the host's bound decides on the pieces
+        cache.max_len = bound
+        got = ops.kv8_attn(q, cache, new=new)
+        assert bool((got[0] == 0).all()) and bool((got[1, 1:] == 0).all())
+        assert torch.isnan(got[1, 0]).all() and torch.isfinite(got[2]).all()
+
+
+@pytest.mark.parametrize("n", [1, 64])
+@pytest.mark.parametrize("total", [200, 2900])
+def test_a_nan_value_whose_weight_underflows_is_not_lost(total, n):
+    """Token 3's score lies some hundred below the others': its weight is zero in f32, and zero times NaN is NaN in every
+    launch shape."""
+    from vit_amd import ops
+    hd = 64
+    k, v, q = (torch.ones(1, m, 1, hd, dtype=BF16) for m in (total, total, n))
+    k[0, :64] = -4.0                                           # whole blocks apart: waves and pieces of their own
+    v[0, 3, 0, 7] = float("nan")
+    got = ops.kv8_attn(q.cuda() * 4, cache_of(k, v), scale=1.0)
+    assert torch.isnan(got[0, :, 0, 7]).all()
+    got[..., 7] = 1.0
+    assert bool((got == 1.0).all())

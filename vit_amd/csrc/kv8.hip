@@ -181,6 +181,12 @@ VA_DEVINL float groups_max(float x) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// What a part's sums count in the whole: 0 where the maximum ignored all it saw, nothing or NaN alone.  The sums are added with
+// that factor too: those of nothing are zeros, and a NaN stays NaN.
+VA_DEVINL float part_factor(float mx, float top, float scale2) {
+    return mx == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((mx - top) * scale2);
+}
+
 // Softmax weights of one 64-key tile for 16 queries and the rescaled running state.  s[kt] = raw scores of keys 16 kt + 4 g + r;
 // pf[u] = the tile's P^T operand for keys 32 u ..+31.  The running maximum is one of raw scores (the scale is positive), the
 // scale goes into the exponent's multiply-add.
@@ -392,14 +398,12 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Cache c, AttnArgs a)
         f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = sml[w][0][row] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((sml[w][0][row] - top) * a.scale2);
+            const float f = part_factor(sml[w][0][row], top, a.scale2);
             total = fmaf(f, sml[w][1][row], total);
-            if (f != 0.f) acc += f * *(const f32x4_t*)(so + (w * 16 + row) * OSTR + col);
+            acc += f * *(const f32x4_t*)(so + (w * 16 + row) * OSTR + col);
         }
         if (a.splits == 1) {
-            const float inv = total > 0.f || total != total ? 1.f / total : 0.f;        // nothing seen: zeros
-            acc *= inv;
-            if (total == 0.f) acc = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            acc *= total == 0.f ? 0.f : 1.f / total;        // nothing seen: zeros
             bf16_t* dst = a.out + (((int64_t)b * a.n + row / a.G) * a.H * a.G + (int64_t)h * a.G + row % a.G) * HD + col;
             *(u32x2_t*)dst = (u32x2_t){pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
         } else {
@@ -601,9 +605,7 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a) {
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
     float total = 0.f;
     for (int s = 0; s < a.splits; ++s) {
-        const float mx = a.part_ml[2 * (s * all + idx)];
-        if (mx == NEG_INF) continue;
-        const float f = __builtin_amdgcn_exp2f((mx - top) * a.scale2);
+        const float f = part_factor(a.part_ml[2 * (s * all + idx)], top, a.scale2);
         total = fmaf(f, a.part_ml[2 * (s * all + idx) + 1], total);
         acc += f * *(const f32x4_t*)(a.part_o + (s * all + idx) * HD + col);
     }
