@@ -87,3 +87,25 @@ def test_a_nan_value_whose_weight_underflows_is_not_lost(total, n):
     assert torch.isnan(got[0, :, 0, 7]).all()
     got[..., 7] = 1.0
     assert bool((got == 1.0).all())
+
+
+@pytest.mark.parametrize("heads,group", [(512, 1), (1, 1024)])
+def test_a_maximum_that_stays_fades_nothing(heads, group):
+    """All keys alike, scores of some thousand: every weight is the same, so the result is the share of values that are one
+    (a half), however many tiles come after the one that set the maximum.  Few rows, many heads: one piece of the keys, four
+    waves; many rows: one workgroup walks all 512 tiles.  A weight is rounded to bf16 and so is the result: 2^-8 of it each."""
+    from vit_amd import ops
+    hd, total, n = 64, 32768, 1 if group == 1 else 64
+    code = lambda x: int(torch.tensor(x).to(torch.float8_e4m3fn).view(torch.uint8))      # noqa: E731
+    k8 = torch.full((1, heads, total, hd), code(3.5), dtype=torch.uint8, device="cuda")
+    v8 = torch.zeros(1, heads, total, hd, dtype=torch.uint8, device="cuda")
+    v8[:, :, :total // 2] = code(1.0)
+    ones = torch.ones(1, heads, total // 64, device="cuda")
+    opened = torch.zeros(1, heads, 64, hd, dtype=BF16, device="cuda")
+    cache = ops.KVCache8(k8.view(torch.float8_e4m3fn), v8.view(torch.float8_e4m3fn), ones, ones.clone(), opened, opened.clone(),
+                         torch.full((1,), total, dtype=torch.int32, device="cuda"))
+    heights = 3.0 + torch.arange(heads * group, device="cuda") % 32 / 64.0               # exact in bf16, other scores for each
+    q = heights.view(1, 1, -1, 1).expand(1, n, heads * group, hd).contiguous().to(BF16)
+    out = ops.kv8_attn(q, cache, scale=37.0).float()
+    worst = (out - 0.5).abs().max().item()
+    assert worst <= 2 * 2.0 ** -8 * 0.5 + 1e-5, worst

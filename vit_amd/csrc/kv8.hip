@@ -184,14 +184,18 @@ VA_DEVINL float groups_max(float x) {
 // What a part's sums count in the whole: 0 where the maximum ignored all it saw, nothing or NaN alone.  The sums are added with
 // that factor too: those of nothing are zeros, and a NaN stays NaN.
 VA_DEVINL float part_factor(float mx, float top, float scale2) {
-    return mx == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((mx - top) * scale2);
+#pragma clang fp contract(off)
+    return mx == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mx * scale2 - top * scale2);     // bases rounded as in tile_softmax
 }
 
 // Softmax weights of one 64-key tile for 16 queries and the rescaled running state.  s[kt] = raw scores of keys 16 kt + 4 g + r;
 // pf[u] = the tile's P^T operand for keys 32 u ..+31.  The running maximum is one of raw scores (the scale is positive), the
-// scale goes into the exponent's multiply-add.
+// scale goes into the exponent's multiply-add.  The sums so far stand on the rounded product of the old maximum and the scale,
+// so the factor to the new base is formed from two such products: exactly 1 while the maximum stays, however many tiles follow
+// (a multiply-add in its place left the product's rounding error in it, once per tile).
 template <bool MASK>
 VA_DEVINL float tile_softmax(f32x4_t (&s)[4], int key0, int g4, int limit, float scale2, float& mx, float& sum, bf16x8_t (&pf)[2]) {
+#pragma clang fp contract(off)
     float top = NEG_INF;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt)
@@ -203,7 +207,7 @@ VA_DEVINL float tile_softmax(f32x4_t (&s)[4], int key0, int g4, int limit, float
     top = groups_max(top);
     const float now = fmaxf(mx, top);
     const float base = now == NEG_INF ? 0.f : now * scale2;     // nothing seen yet: every weight is exp2(-inf) = 0
-    const float fade = __builtin_amdgcn_exp2f(fmaf(mx, scale2, -base));
+    const float fade = __builtin_amdgcn_exp2f(mx * scale2 - base);
     mx = now;
     float add = 0.f;
     uint32_t pk[4][2];
