@@ -422,6 +422,14 @@ def _note_torch_path(x: torch.Tensor, who: str) -> None:
                   "torch.no_grad().", RuntimeWarning, stacklevel=3)
 
 
+def _as_torch_made_it(module: nn.Module, kind) -> bool:
+    """True where calling `module` does what `kind` does and nothing else: no subclass or own forward, no hooks (of the module
+    or of all modules), not compiled.  Only then may a kernel take its place."""
+    return (type(module) is kind and "forward" not in vars(module) and not nn.modules.module._has_any_global_hook()
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
+            and getattr(module, "_compiled_call_impl", None) is None)
+
+
 class GatedDeltaLayer(nn.Module):
     """Gated delta-rule memory layer (swm:431-555).  What is computed is the sequential recurrence: the form inference uses
     and the one the reference's other ("parallel") path fails to reproduce.  On the device (f32, head dim 64 or 128) short
@@ -465,6 +473,14 @@ class GatedDeltaLayer(nn.Module):
             outs.append(torch.einsum("bhij,bhj->bhi", state, qt))
         return torch.stack(outs, dim=1), state
 
+    def _plain_output_stage(self, v_gate) -> bool:
+        """Whether the output stage's kernel computes what silu and o_norm would: the modules as __init__ makes them, without
+        hooks, f32, at most 4096 wide."""
+        norm, inner = self.o_norm, self.num_heads * self.head_dim
+        return (_as_torch_made_it(norm, nn.LayerNorm) and _as_torch_made_it(self.silu, nn.SiLU) and inner <= 4096
+                and norm.normalized_shape == (inner,) and v_gate.dtype == torch.float32
+                and all(p is not None and p.dtype == torch.float32 and p.device == v_gate.device for p in (norm.weight, norm.bias)))
+
     def forward(self, x, state=None, use_parallel=None):
         B, L, _ = x.shape
         H, Dh = self.num_heads, self.head_dim
@@ -490,9 +506,13 @@ class GatedDeltaLayer(nn.Module):
                     # the convolutions leave (batch, channel, time) order behind
                     out, new_state = module_ops.gated_delta(*(t.contiguous().view(B, L, H, Dh) for t in (q, k, v)), alpha, beta,
                                                             state)
-                    if H * Dh <= 4096:
-                        out = module_ops.gated_layernorm(out.view(B, L, H * Dh), v_gate, self.g_proj(x), self.o_norm.weight,
-                                                         self.o_norm.bias, self.o_norm.eps)
+                    if self._plain_output_stage(v_gate):
+                        g = self.g_proj(x)
+                        if g.shape == v_gate.shape and g.dtype == torch.float32:
+                            out = module_ops.gated_layernorm(out.view(B, L, H * Dh), v_gate, g, self.o_norm.weight,
+                                                             self.o_norm.bias, self.o_norm.eps)
+                        else:
+                            out = self.o_norm((out * v_gate.view(B, L, H, Dh)).reshape(B, L, -1) * self.silu(g))
                         return self.o_proj(out), new_state
             else:
                 out, new_state = self._sequential_gated_delta(q.view(B, L, H, Dh), k.view(B, L, H, Dh), v.view(B, L, H, Dh),
