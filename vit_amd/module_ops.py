@@ -243,9 +243,15 @@ def _addressless(*grads) -> bool:
     return False
 
 
-def by_torch_alone() -> bool:
-    """True where every operation must be torch's own: torch.func transforms, forward-mode derivatives, autocast."""
-    return _functorch_active() or torch.autograd.forward_ad._current_level >= 0 or torch.is_autocast_enabled("cuda")
+_PLAIN = (torch.Tensor, torch.nn.Parameter, type(None))
+
+
+def by_torch_alone(*tensors) -> bool:
+    """True where every operation must be torch's own: compilation, export and tracing, dispatch modes (fake tensors, make_fx),
+    tensors of a subclass among `tensors`, torch.func transforms, forward-mode derivatives, autocast."""
+    return (torch.compiler.is_compiling() or torch.jit.is_tracing() or torch._C._len_torch_dispatch_stack() > 0
+            or any(type(t) not in _PLAIN for t in tensors) or _functorch_active()
+            or torch.autograd.forward_ad._current_level >= 0 or torch.is_autocast_enabled("cuda"))
 
 
 def _torch_grads(formula, inputs, needed, grads):

@@ -500,7 +500,9 @@ class GatedDeltaLayer(nn.Module):
             k = F.normalize(self.silu(self._causal_conv(self.k_conv1d, self.k_proj(x))), p=2, dim=-1)
             v = self.silu(self._causal_conv(self.v_conv1d, self.v_proj(x)))
             v, v_gate = v.chunk(2, dim=-1)
-            if x.is_cuda and q.dtype == torch.float32 and Dh in (64, 128) and not module_ops.by_torch_alone():
+            if (Dh in (64, 128) and all(t.is_cuda and t.dtype == torch.float32 for t in (x, q, k, v, alpha, beta))
+                    and (state is None or state.dtype in (torch.float32, torch.bfloat16, torch.float16))
+                    and not module_ops.by_torch_alone(x, q, k, v, alpha, beta, state, *self.o_norm.parameters())):
                 state = None if state is None else state.expand(B, H, Dh, Dh)
                 with torch.cuda.device(x.device):
                     # the convolutions leave (batch, channel, time) order behind
