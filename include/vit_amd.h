@@ -310,7 +310,7 @@ int va_gated_delta_seq(const float* q, const float* k, const float* v, const flo
  * va_gated_delta_seq), for whole sequences, with its gradient, and for one token:
  *     S_t = a_t S_{t-1} (I - b_t k_t k_t^T) + b_t v_t k_t^T,   o_t = S_t q_t
  * q, k, v: rows of token (b, t) `ld*` elements apart (a multiple of 4, at least H*hd), heads side by side, all f32 or all
- * bf16 (is_bf16; 8-byte alignment is enough then); alpha, beta: contiguous f32 [B,L,H]; states f32 [B,H,hd,hd] (rows = value
+ * bf16 (is_bf16; 8-byte alignment is enough then, for d_out too); alpha, beta: contiguous f32 [B,L,H]; states f32 [B,H,hd,hd] (rows = value
  * index); out / gradients of q, k, v: contiguous [B,L,H,hd] of the inputs' type.  hd 64 or 128.  Products and states are
  * f32 whatever the type.  A non-finite value reaches what it does in the recurrence (rows that meet one are
  * formed again token by token); in the gradient it spreads over the 64-token chunk it lies in, earlier tokens included.

@@ -125,3 +125,66 @@ def test_hooks_of_all_modules_see_the_norm():
     finally:
         handle.remove()
     assert "LayerNorm" in seen
+
+
+def off_by_one(t):
+    """The same numbers contiguous, one element past a 16-byte boundary."""
+    flat = torch.empty(t.numel() + 8, dtype=t.dtype, device=t.device)
+    view = flat[1:1 + t.numel()].view(t.shape)
+    view.copy_(t.detach())
+    assert view.data_ptr() % 16 != 0 and view.is_contiguous()
+    return view
+
+
+@gpu
+def test_a_norm_whose_parameters_are_views_of_a_flat_buffer():
+    def flatten(m):
+        for name in ("weight", "bias"):
+            p = getattr(m.o_norm, name)
+            if p.is_cuda:
+                setattr(m.o_norm, name, nn.Parameter(off_by_one(p)))
+    layer = layer_of()
+    dev = layer.cuda()
+    flatten(dev)
+    assert dev.o_norm.weight.data_ptr() % 16 != 0
+    ref = copy.deepcopy(layer).double().cpu()
+    x = R.hashed_uniform("ly.x", (2, 9, 96), 1.0)
+    s = R.hashed_uniform("ly.s", (2, 2, 64, 64), 0.2)
+    sd = off_by_one(s.cuda()).requires_grad_()
+    sr = s.double().requires_grad_()
+    got, want = dev(x.cuda(), sd), ref(x.double(), sr)
+    assert rel(got[0], want[0]) < 1e-4 and rel(got[1], want[1]) < 1e-4
+    grads = torch.autograd.grad(got[0].sum() + got[1].pow(2).sum(), [dev.o_norm.weight, dev.o_norm.bias, sd])
+    wanted = torch.autograd.grad(want[0].sum() + want[1].pow(2).sum(), [ref.o_norm.weight, ref.o_norm.bias, sr])
+    for g, w in zip(grads, wanted):
+        assert rel(g, w) < 1e-4
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_and_operands_off_a_16_byte_boundary(dtype):
+    """The differentiable operators take gradients, states and rows wherever they lie."""
+    from vit_amd import module_ops, ops
+    B, L, H, hd = 2, 70, 2, 64
+    q, k, v = (R.hashed_uniform(f"of.{n}", (B, L, H, hd), 0.1).to(dtype).cuda() for n in "qkv")
+    a, b = R.hashed_uniform("of.a", (B, L, H), 0.2, 0.8).cuda(), R.hashed_uniform("of.b", (B, L, H), 0.5, 0.5).cuda()
+    s = R.hashed_uniform("of.s", (B, H, hd, hd), 0.4).cuda()
+    go, gs = R.hashed_uniform("of.go", (B, L, H, hd), 1.0).to(dtype).cuda(), R.hashed_uniform("of.gs", s.shape, 0.5).cuda()
+    results = []
+    for state, d_out, d_state in ((s, go, gs), (off_by_one(s), off_by_one(go), off_by_one(gs))):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, a, b, state)]
+        results.append(torch.autograd.grad(module_ops.gated_delta(*leaves), leaves, (d_out, d_state)))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+    rows = [R.hashed_uniform(f"of.r{n}", (9, 96), 1.0).to(dtype).cuda() for n in range(3)]
+    scale, shift = (R.hashed_uniform(f"of.{n}", (96,), 0.5, 1.0).cuda() for n in ("gamma", "beta"))
+    dy, results = R.hashed_uniform("of.dy", (9, 96), 1.0).to(dtype).cuda(), []
+    for move in (lambda t: t, off_by_one):
+        leaves = [move(t).detach().requires_grad_() for t in (*rows, scale, shift)]
+        y = module_ops.gated_layernorm(*leaves)
+        results.append([y, *torch.autograd.grad(y, leaves, move(dy))])
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+    if dtype == torch.bfloat16:                                # 8 bytes are enough for bf16 rows, the gradient's too
+        flat = torch.empty(go.numel() + 4, dtype=dtype, device="cuda")
+        moved = flat[4:].view(go.shape).copy_(go)
+        for x, y in zip(ops.gated_delta_bwd(moved, gs, q, k, v, a, b, s), ops.gated_delta_bwd(go, gs, q, k, v, a, b, s)):
+            assert torch.equal(x, y)

@@ -1418,8 +1418,8 @@ extern "C" int va_gated_delta_bwd(const void* d_out, const float* d_state, const
     const DeltaArgs d = {q, k, v, ldq, ldk, ldv, alpha, beta, B, L, H, hd, is_bf16 != 0};
     VA_TRY(delta_check("va_gated_delta_bwd", d));
     VA_CHECK_ARG(d_out && dq && dk && dv && dalpha && dbeta && workspace, "va_gated_delta_bwd: null operand");
-    VA_CHECK_ARG(((uintptr_t)state_in | (uintptr_t)d_state | (uintptr_t)d_state_in | (uintptr_t)workspace | (uintptr_t)kept |
-                  (uintptr_t)d_out) % 16 == 0,
+    VA_CHECK_ARG(((uintptr_t)state_in | (uintptr_t)d_state | (uintptr_t)d_state_in | (uintptr_t)workspace | (uintptr_t)kept) % 16 == 0 &&
+                     (uintptr_t)d_out % (d.bf16 ? 8 : 16) == 0,       // four elements of d_out are read at a time
                  "va_gated_delta_bwd: misaligned state, gradient or workspace");
     if (hd == 128)
         return d.bf16 ? delta_bwd<128, bf16_t>(d, d_out, d_state, state_in, dq, dk, dv, dalpha, dbeta, d_state_in, workspace, kept, stream)

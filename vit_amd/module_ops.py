@@ -279,6 +279,12 @@ def _delta_by_torch(q, k, v, alpha, beta, state):
     return torch.stack(outs, 1).to(dtype), state
 
 
+def _dense(t):
+    """Contiguous and on the 16-byte boundary that the kernels' wide loads want; a copy where a view is not."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class GatedDeltaFn(torch.autograd.Function):
     """Gated delta rule over a sequence (swm:523-555) with the gradients of every input and of the carried state."""
 
@@ -299,17 +305,17 @@ class GatedDeltaFn(torch.autograd.Function):
             return (None,) * 6
         if torch.is_grad_enabled() or _addressless(d_out, d_state):
             return _torch_grads(_delta_by_torch, (q, k, v, alpha, beta, state), ctx.needs_input_grad, (d_out, d_state))
-        d_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if d_out is None else d_out.contiguous()
+        d_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if d_out is None else _dense(d_out)
         want = state is not None and ctx.needs_input_grad[5]
-        grads = ops.gated_delta_bwd(d_out, None if d_state is None else d_state.contiguous(), q, k, v, alpha, beta, state, want,
+        grads = ops.gated_delta_bwd(d_out, None if d_state is None else _dense(d_state), q, k, v, alpha, beta, state, want,
                                     kept)
         return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad))
 
 
 def gated_delta(q, k, v, alpha, beta, state=None):
-    """Differentiable `ops.gated_delta_fwd`: (out, new state).  alpha, beta and the state are made f32 and contiguous."""
+    """Differentiable `ops.gated_delta_fwd`: (out, new state).  alpha, beta and the state are made f32, contiguous and aligned."""
     alpha, beta = alpha.to(F32).contiguous(), beta.to(F32).contiguous()
-    state = None if state is None else state.to(F32).contiguous()
+    state = None if state is None else _dense(state.to(F32))
     return GatedDeltaFn.apply(q, k, v, alpha, beta, state)
 
 
@@ -335,7 +341,7 @@ class GatedLayerNormFn(torch.autograd.Function):
                 return (torch.nn.functional.layer_norm(x, x.shape[-1:], gamma, beta, ctx.eps).to(o.dtype),)
             return _torch_grads(formula, (o, gate, g, gamma, beta), ctx.needs_input_grad[:5], (dy,)) + (None,)
         width = o.shape[-1]
-        grads = ops.gated_layernorm_bwd(*(t.reshape(-1, width) for t in (dy.contiguous(), o, gate, g)), gamma, mean, rstd)
+        grads = ops.gated_layernorm_bwd(*(t.reshape(-1, width) for t in (_dense(dy), o, gate, g)), gamma, mean, rstd)
         grads = [x.view(o.shape) for x in grads[:3]] + list(grads[3:])
         return tuple(x if need else None for x, need in zip(grads, ctx.needs_input_grad)) + (None,)
 
@@ -344,4 +350,4 @@ def gated_layernorm(o, gate, g, gamma, beta, eps: float = 1e-5):
     """Differentiable `ops.gated_layernorm_fwd` over the last dimension; o, gate, g of one shape and type (f32 or bf16)."""
     if gate.shape != o.shape or g.shape != o.shape:
         raise ValueError("gated_layernorm: o, gate and g must share one shape")
-    return GatedLayerNormFn.apply(o.contiguous(), gate.contiguous(), g.contiguous(), gamma, beta, float(eps))
+    return GatedLayerNormFn.apply(_dense(o), _dense(gate), _dense(g), _dense(gamma), _dense(beta), float(eps))
