@@ -20,6 +20,7 @@
 // (the last line needs no division by a decay, so decays of zero are ordinary numbers; the decays themselves are running
 // products, never differences of logarithms).  delta_rscan_kernel walks backwards, then delta_grad_kernel takes the chunks in
 // parallel, both from the forward's T^T, P^T, U and chunk states (kept by it, or formed again by its two kernels).
+// Heads with a result that is not finite go through delta_grad_by_token_kernel behind them.
 //
 // Numbers on the matrix pipe.  The bf16 instruction (16x16x32) does sixteen times the products of the f32 one (16x16x4) per
 // cycle, so the scans split every f32 operand into three bf16 numbers, x = x0 + x1 + x2 with |x1| <= 2^-8 |x| and
@@ -899,7 +900,7 @@ __global__ __launch_bounds__(512) void delta_grad_kernel(const T* __restrict__ Q
                                                          const float* __restrict__ US, const float* __restrict__ RS,
                                                          const float* __restrict__ MS, const float* __restrict__ GS,
                                                          T* __restrict__ DQ, T* __restrict__ DK, float* __restrict__ DALPHA,
-                                                         float* __restrict__ DBETA, int L, int H, int NC) {
+                                                         float* __restrict__ DBETA, uint8_t* __restrict__ BAD, int L, int H, int NC) {
     constexpr int CGS = 4, NR = 2, NN = HD / 64;   // column groups; row and column tiles of a wave
     typedef GradLds<HD> S;
     extern __shared__ __align__(16) char lds[];
@@ -1113,6 +1114,7 @@ __global__ __launch_bounds__(512) void delta_grad_kernel(const T* __restrict__ Q
                 }
     }
     const ChunkOf<T> dqc = chunk_of((const T*)DQ + first, dense, left), dkc = chunk_of((const T*)DK + first, dense, left);
+    float seen = 0.f;                              // NaN with any result that is not finite
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -1122,6 +1124,7 @@ __global__ __launch_bounds__(512) void delta_grad_kernel(const T* __restrict__ Q
                 const int i = 16 * (r0 + n) + g4 + r;
                 dqc.put(i, col + 16 * x, X[n][x][r]);
                 dkc.put(i, col + 16 * x, Z[n][x][r]);
+                seen = fmaf(X[n][x][r], 0.f, fmaf(Z[n][x][r], 0.f, seen));
             }
     // da_t: D[t][i] = sum_{j < t} g_{t-1,j} d(g_ij) + g_{t-1} d(g_i), weighted with g_it and summed over i >= t.  The first four
     // waves take a row tile of t each.
@@ -1158,10 +1161,14 @@ __global__ __launch_bounds__(512) void delta_grad_kernel(const T* __restrict__ Q
             for (int off = 1; off < 16; off <<= 1) da[r] += __shfl_xor(da[r], off);
             const int tt = 16 * wave + g4 + r;
             if (m == 0 && tt < left) DALPHA[(b * L + t0 + tt) * H + h] = da[r];
+            seen = fmaf(da[r], 0.f, seen);
         }
-        if (lane < 16 && t < left)
-            DBETA[(b * L + t0 + t) * H + h] = sdb[0][t] + sdb[1][t] + sdb[2][t] + sdb[3][t] + srv[t] - sg[t] * sky[t];
+        const float db = sdb[0][t] + sdb[1][t] + sdb[2][t] + sdb[3][t] + srv[t] - sg[t] * sky[t];
+        if (lane < 16 && t < left) DBETA[(b * L + t0 + t) * H + h] = db;
+        seen = fmaf(db, 0.f, seen);
     }
+    const bool bad = __any(seen != seen);
+    if (lane == 0) BAD[ci * 8 + wave] = bad;
 }
 
 template <typename T> struct elem;
@@ -1175,6 +1182,139 @@ template <> struct elem<bf16_t> {
     static VA_DEVINL float get(const bf16_t* p) { return bf16_to_f32(*p); }
     static VA_DEVINL void put(bf16_t* p, float x) { *p = f32_to_bf16(x); }      // the output's own type: one rounding
 };
+
+// ---------------------------------------------------------------------------------------------------------------
+// The gradients of a head with a result that is not finite, token by token: there a product with a zero of the chunked form
+// (a weight above the diagonal, a row behind the sequence) has turned a bad number of one token into bad gradients of others.
+// A bad dv or state gradient always shows in dq, dk or a gate of its chunk too, which R and G enter.  One workgroup per head,
+// HD / 16 waves of 16 rows of the state S and of G = dL/dS, four lanes to a row; with P = S_{t-1}, u = b (v - a P k), walking
+// back from the last token
+//     dq = S_t^T do,   G += do q^T,   dv = b G k,   da = <G, P - b (P k) k^T>,   db = (G k).(v - a P k),
+//     dk = G^T u - a b P^T (G k),     G <- a (G - b (G k) k^T).
+// P is formed anew from the chunk's first state for each token (GS, whose chunked contents are of no use, holds those): rare, so
+// this trades time for memory (32 heads x 1290 tokens of f32, head dim 128, all bad: 37 ms).  Heads whose results are finite
+// leave at once.
+template <int HD, typename T>
+__global__ __launch_bounds__(4 * HD) void delta_grad_by_token_kernel(const T* __restrict__ Q, const T* __restrict__ K,
+                                                                     const T* __restrict__ V, Rows rq, Rows rk, Rows rv,
+                                                                     const T* __restrict__ DO, const float* __restrict__ ALPHA,
+                                                                     const float* __restrict__ BETA, const float* __restrict__ STATE_IN,
+                                                                     const float* __restrict__ DSTATE, const uint64_t* __restrict__ BAD,
+                                                                     T* __restrict__ DQ, T* __restrict__ DK, T* __restrict__ DV,
+                                                                     float* __restrict__ DALPHA, float* __restrict__ DBETA,
+                                                                     float* __restrict__ DSTATE_IN, float* GS, int L, int H, int NC) {
+    constexpr int W = HD / 16, N = HD / 16;        // waves; groups of four columns of a lane
+    __shared__ float part[2][W][HD];               // column sums of a wave's rows: dq, dk
+    __shared__ float gate[2][W];                   // da, db
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = 16 * wave + (lane & 15), col = (lane >> 4) * (HD / 4);
+    const int64_t bh = blockIdx.x, b = bh / H, h = bh % H;
+    int any = 0;
+    for (int c = tid; c < NC; c += 4 * HD) any |= BAD[bh * NC + c] != 0;
+    if (!__syncthreads_or(any)) return;
+    const T *q = Q + rq.at(b, L, 0, h, HD), *k = K + rk.at(b, L, 0, h, HD), *v = V + rv.at(b, L, 0, h, HD);
+    const int64_t first = b * L * H + h;
+    const int64_t at = bh * HD * HD + row * HD + col;              // this lane's part of a state
+    float* starts = GS + bh * NC * HD * HD + row * HD + col;
+    f32x4_t S[N], G[N], kt[N], qt[N];
+    auto over_row = [](float x) {
+        x += __shfl_xor(x, 16);
+        return x + __shfl_xor(x, 32);
+    };
+    auto over_rows = [](float x) {
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) x += __shfl_xor(x, off);
+        return x;
+    };
+    auto row_of = [&](const T* p, int64_t ld, int t, f32x4_t (&to)[N]) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) to[n] = elem<T>::load4(p + t * ld + col + 4 * n);
+    };
+    auto dot = [&](const f32x4_t (&x)[N], const f32x4_t (&y)[N]) {
+        float d = 0.f;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d = fmaf(x[n][r], y[n][r], d);
+        return over_row(d);
+    };
+    auto forward = [&](int t) {                    // S_{t-1} -> S_t
+        const float a = ALPHA[first + (int64_t)t * H], bt = BETA[first + (int64_t)t * H];
+        row_of(k, rk.ld, t, kt);
+        const float u = bt * (elem<T>::get(v + t * rv.ld + row) - a * dot(S, kt));
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[n][r] = fmaf(u, kt[n][r], a * S[n][r]);
+    };
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        S[n] = G[n] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+        if (STATE_IN != nullptr) S[n] = *(const f32x4_t*)(STATE_IN + at + 4 * n);
+        if (DSTATE != nullptr) G[n] = *(const f32x4_t*)(DSTATE + at + 4 * n);
+    }
+#pragma unroll 1
+    for (int c = 0; c < NC; ++c) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) *(f32x4_t*)(starts + (int64_t)c * HD * HD + 4 * n) = S[n];
+        if (c + 1 < NC)
+#pragma unroll 1
+            for (int t = c * DC; t < (c + 1) * DC; ++t) forward(t);
+    }
+#pragma unroll 1
+    for (int t = L - 1; t >= 0; --t) {
+        const int c = t / DC;
+#pragma unroll
+        for (int n = 0; n < N; ++n) S[n] = *(const f32x4_t*)(starts + (int64_t)c * HD * HD + 4 * n);
+#pragma unroll 1
+        for (int s = c * DC; s < t; ++s) forward(s);
+        const int64_t token = first + (int64_t)t * H;
+        const float a = ALPHA[token], bt = BETA[token];
+        row_of(k, rk.ld, t, kt);
+        row_of(q, rq.ld, t, qt);
+        const float dov = elem<T>::get(DO + token * HD + row), sk = dot(S, kt), w = elem<T>::get(v + t * rv.ld + row) - a * sk, u = bt * w;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float x = over_rows(fmaf(u, kt[n][r], a * S[n][r]) * dov);
+                if ((lane & 15) == 0) part[0][wave][col + 4 * n + r] = x;
+                G[n][r] = fmaf(dov, qt[n][r], G[n][r]);
+            }
+        const float gk = dot(G, kt);
+        float da = 0.f;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                da = fmaf(G[n][r], fmaf(-bt * sk, kt[n][r], S[n][r]), da);
+                const float x = over_rows(fmaf(G[n][r], u, -(a * bt) * gk * S[n][r]));
+                if ((lane & 15) == 0) part[1][wave][col + 4 * n + r] = x;
+                G[n][r] = a * fmaf(-bt * gk, kt[n][r], G[n][r]);
+            }
+        if (lane < 16) elem<T>::put(DV + token * HD + row, bt * gk);
+        da = over_row(over_rows(da));
+        const float db = over_rows(gk * w);        // the same in the four lanes of a row
+        if (lane == 0) gate[0][wave] = da, gate[1][wave] = db;
+        __syncthreads();
+        if (tid < 2 * HD) {
+            float x = 0.f;
+#pragma unroll
+            for (int n = 0; n < W; ++n) x += part[tid / HD][n][tid % HD];
+            elem<T>::put((tid < HD ? DQ : DK) + token * HD + tid % HD, x);
+        }
+        if (tid < 2) {
+            float x = 0.f;
+#pragma unroll
+            for (int n = 0; n < W; ++n) x += gate[tid][n];
+            (tid == 0 ? DALPHA : DBETA)[token] = x;
+        }
+        __syncthreads();                           // the sums have been read
+    }
+    if (DSTATE_IN != nullptr) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) *(f32x4_t*)(DSTATE_IN + at + 4 * n) = G[n];
+    }
+}
 
 // ---------------------------------------------------------------------------------------------------------------
 // One token: S <- a S + u k^T, u = b (v - a S k), o = S q = a (S_old q) + u (k.q).  The state is read and written once and
@@ -1333,7 +1473,7 @@ int launch_rscan(const DeltaArgs& d, const Work<T>& w, const void* d_out, const 
 constexpr int64_t OPERAND_BYTES = BLK * BFRAG * 2;
 int64_t own_chunk_bytes() { return 6 * OPERAND_BYTES + 2 * DC * 4; }
 int64_t kept_chunk_bytes(int64_t hd) { return 2 * DC * 4 + 6 * OPERAND_BYTES + DC * hd * 4 + hd * hd * 4; }
-int64_t bwd_chunk_bytes(int64_t hd) { return DC * hd * 4 + hd * hd * 4; }
+int64_t bwd_chunk_bytes(int64_t hd) { return DC * hd * 4 + hd * hd * 4 + 16; }      // 8 of the 16: a flag per wave
 
 template <int HD, typename T>
 int delta_fwd(const DeltaArgs& d, const float* state_in, void* out, float* state_out, float* ws, float* kept, hipStream_t stream) {
@@ -1358,6 +1498,7 @@ int delta_bwd(const DeltaArgs& d, const void* d_out, const float* d_state, const
     Work<T> w = {};
     Pieces own = {(char*)ws};
     float *rs = own.take<float>(n * DC * HD), *gs = own.take<float>(n * HD * HD);
+    uint8_t* bad = own.take<uint8_t>(n * 8);
     if (kept != nullptr) {
         Pieces k = {(char*)kept};
         take_kept(d, k, w);
@@ -1373,9 +1514,14 @@ int delta_bwd(const DeltaArgs& d, const void* d_out, const float* d_state, const
     const auto fn = delta_grad_kernel<HD, T>;
     VA_TRY(reserve_lds("va_gated_delta_bwd", (const void*)fn, lds));
     hipLaunchKernelGGL(fn, dim3((unsigned)n), dim3(512), lds, stream, (const T*)d.q, (const T*)d.k, (const T*)d.v, Rows{d.ldq},
-                       Rows{d.ldk}, Rows{d.ldv}, (const T*)d_out, d.alpha, d.beta, w.us, rs, w.ms, gs, (T*)dq, (T*)dk, dalpha, dbeta,
+                       Rows{d.ldk}, Rows{d.ldv}, (const T*)d_out, d.alpha, d.beta, w.us, rs, w.ms, gs, (T*)dq, (T*)dk, dalpha, dbeta, bad,
                        (int)d.L, (int)d.H, (int)d.chunks());
     VA_CHECK_LAUNCH("va_gated_delta_bwd (gradients)");
+    hipLaunchKernelGGL((delta_grad_by_token_kernel<HD, T>), dim3((unsigned)(d.B * d.H)), dim3(4 * HD), 0, stream, (const T*)d.q,
+                       (const T*)d.k, (const T*)d.v, Rows{d.ldq}, Rows{d.ldk}, Rows{d.ldv}, (const T*)d_out, d.alpha, d.beta, state_in,
+                       d_state, (const uint64_t*)bad, (T*)dq, (T*)dk, (T*)dv, dalpha, dbeta, d_state_in, gs, (int)d.L, (int)d.H,
+                       (int)d.chunks());
+    VA_CHECK_LAUNCH("va_gated_delta_bwd (token by token)");
     return VA_OK;
 }
 

@@ -609,8 +609,8 @@ def gated_delta_fwd(q, k, v, alpha, beta, state=None, keep: bool = False):
     """The recurrence of `gated_delta_seq` in its chunked form (products over 64 tokens on the matrix pipe): q, k, v f32 or
     bf16 [B,L,H,hd] (rows any constant stride apart), hd 64 or 128; alpha, beta f32 [B,L,H]; state f32 [B,H,hd,hd] or None
     -> (out [B,L,H,hd] of q's type, new state f32).  A head's sequence that meets a non-finite value is formed again token
-    by token, so earlier tokens stay finite (not their gradients: there it spreads over its chunk of 64).  keep=True: a third
-    result, what `gated_delta_bwd` otherwise computes again (about 2 KiB per token and head of 128)."""
+    by token, and so are a head's gradients, so it reaches what it does in the recurrence and nothing else.  keep=True: a
+    third result, what `gated_delta_bwd` otherwise computes again (about 2 KiB per token and head of 128)."""
     lds = _delta_operands("gated_delta_fwd", q, k, v, alpha, beta, state, 2)
     B, L, H, hd = q.shape
     lib = _lib.load()
