@@ -109,3 +109,43 @@ def test_a_maximum_that_stays_fades_nothing(heads, group):
     out = ops.kv8_attn(q, cache, scale=37.0).float()
     worst = (out - 0.5).abs().max().item()
     assert worst <= 2 * 2.0 ** -8 * 0.5 + 1e-5, worst
+
+
+def test_padded_appends_are_refused_only_when_a_stream_is_full(monkeypatch):
+    """The host's bound counts the padding of ragged appends; when it passes the capacity the lengths themselves decide."""
+    from vit_amd import ops
+    B, H, hd, n = 3, 1, 64, 40
+    cache, twin = (ops.KVCache8.empty(B, H, hd, 128, "cuda") for _ in range(2))
+    k, v = tokens(B, n, H, hd, "p.k").cuda(), tokens(B, n, H, hd, "p.v").cuda()
+    counts = [[40, 0, 5], [0, 40, 5], [40, 0, 5], [0, 40, 5], [0, 0, 5], [0, 0, 0], [40, 40, 5]]
+    lens = [0] * B
+    for row in counts:                                         # 280 padded tokens, at most 120 in a stream
+        new = torch.tensor(row, dtype=torch.int32, device="cuda")
+        ops.kv8_append_(cache, k, v, new=new)
+        lens = [x + y for x, y in zip(lens, row)]
+        assert cache.lengths.tolist() == lens and max(lens) <= cache.max_len <= cache.capacity
+        for b, m in enumerate(row):                            # the same tokens, each stream by itself, never padded
+            if m:
+                one = torch.zeros(B, dtype=torch.int32, device="cuda")
+                one[b] = m
+                twin.max_len = max(lens) - m
+                ops.kv8_append_(twin, k[:, :m], v[:, :m], new=one)
+    assert lens == [120, 120, 30]
+    for name in ("k8", "v8", "k_scale", "v_scale", "k_open", "v_open", "lengths"):
+        x, y = getattr(cache, name), getattr(twin, name)
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), name
+    with pytest.raises(ValueError):                            # stream 1 would hold 129
+        ops.kv8_append_(cache, k, v, new=torch.tensor([0, 9, 0], dtype=torch.int32, device="cuda"))
+    assert cache.lengths.tolist() == lens
+    ops.kv8_append_(cache, k, v, new=torch.tensor([8, -3, 40], dtype=torch.int32, device="cuda"))
+    assert cache.lengths.tolist() == [128, 120, 70]
+    with pytest.raises(ValueError):
+        ops.kv8_append_(cache, k[:, :1], v[:, :1])
+    with monkeypatch.context() as m:                           # a capture must not ask the device
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(ValueError):
+            ops.kv8_append_(cache, k, v, new=torch.zeros(B, dtype=torch.int32, device="cuda"))
+        with pytest.raises(RuntimeError):
+            cache.sync_length()
+    cache.lengths.copy_(torch.tensor([3, 70, 0]))
+    assert cache.sync_length() == 70 == cache.max_len

@@ -418,9 +418,9 @@ class KVCache8:
     """Keys and values of `lengths` tokens per stream in 8 bits: e4m3 codes k8, v8 [B, H, capacity, hd] with one f32
     power-of-two scale per block of 64 tokens and head (k_scale, v_scale [B, H, capacity / 64]); the block that is not full yet
     lies in k_open, v_open [B, H, 64, hd] bf16.  A code times its scale is the value it stands for.  `max_len` is the host's
-    upper bound of the lengths (they live on the device): `kv8_append_` raises when it would pass the capacity.  A replayed
-    graph appends without the host: count its tokens into `max_len` yourself; on the device those that pass the capacity are
-    dropped."""
+    upper bound of the lengths (they live on the device); it counts the padding of ragged appends too, `sync_length` brings it
+    down to the longest stream.  A replayed graph appends without the host: count its tokens into `max_len` yourself, or call
+    `sync_length`; on the device those that pass the capacity are dropped."""
 
     def __init__(self, k8, v8, k_scale, v_scale, k_open, v_open, lengths, max_len: Optional[int] = None):
         if k8.dim() != 4 or k8.shape[2] % KV8_BLOCK or 0 in k8.shape:
@@ -462,6 +462,13 @@ class KVCache8:
         self.lengths.zero_()
         self.max_len = 0
 
+    def sync_length(self) -> int:
+        """Set `max_len` to the longest stream's length, which the device is asked for (and waited for)."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("KVCache8.sync_length: not while a graph is captured")
+        self.max_len = int(self.lengths.max())
+        return self.max_len
+
 
 def _token_strides(t: torch.Tensor, name: str, shape) -> Tuple[int, int]:
     """(elements between tokens, between streams) of bf16 [B, n, heads, hd] with the heads of a token side by side."""
@@ -484,7 +491,8 @@ def _new_tokens(new: torch.Tensor, B: int):
 def kv8_append_(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, new: Optional[torch.Tensor] = None) -> KVCache8:
     """Put k, v bf16 [B, n, H, hd] (any token and stream strides) behind the streams' tokens; of stream b only the first
     new[b] (int32 [B] on the device; None: all n).  A block is quantised when its 64 tokens are there, so the codes do not
-    depend on how many tokens came per call."""
+    depend on how many tokens came per call.  Raises where a stream would pass the capacity; while a graph is captured, where
+    the cache's bound and n do (the lengths cannot be read then)."""
     B, H, hd = cache.batch, cache.heads, cache.head_dim
     if k.dim() != 4 or k.shape[1] == 0:
         raise ValueError("kv8_append_: k must be [B, n, H, hd] with at least one token")
@@ -493,11 +501,16 @@ def kv8_append_(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, new: Optional
     ldv, bsv = _token_strides(v, "v", (B, n, H, hd))
     if new is not None:
         _new_tokens(new, B)
-    if cache.max_len + n > cache.capacity:
-        raise ValueError(f"kv8_append_: {n} tokens behind up to {cache.max_len} pass the capacity of {cache.capacity}")
+    after = cache.max_len + n
+    if after > cache.capacity:
+        # the bound counts padding: what the streams would really hold decides, where the device can be asked
+        if not torch.cuda.is_current_stream_capturing():
+            after = int((cache.lengths + (n if new is None else new.clamp(0, n))).max())
+        if after > cache.capacity:
+            raise ValueError(f"kv8_append_: a stream would hold {after} tokens, the capacity is {cache.capacity}")
     check(_lib.load().va_kv8_append(k.data_ptr(), v.data_ptr(), ldk, ldv, bsk, bsv, _p(new), n, *cache.pointers(), B, H, hd,
                                     cache.capacity, _stream()), "va_kv8_append")
-    cache.max_len += n
+    cache.max_len = after
     return cache
 
 
