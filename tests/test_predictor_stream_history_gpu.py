@@ -64,3 +64,22 @@ def test_the_attention_branch_reads_all_earlier_timesteps():
         assert rel(got[:, part], want[:, part]) < REL_TOL, t
         if t > 0:
             assert rel(without[:, part], want[:, part]) > 5 * REL_TOL, t
+
+
+def test_states_that_do_not_fit_are_refused_before_any_block_has_taken_the_tokens():
+    from vit_amd import surgical_world_model as swm
+    model = swm.SurgicalActionConditionedWorldModel(img_size=32, num_frames=4, encoder_depth=1, encoder_heads=16,
+                                                    predictor_depth=2, predictor_heads=8).cuda()
+    B, per = 2, model.tokens_per_frame + 2
+    tokens = R.hashed_uniform("hi.w", (B, per, 1024), 1.0).cuda()
+    steps = 128 // per                                         # timesteps that a cache of two blocks holds
+    for spoil in ("batch", "capacity"):
+        streams = model.new_predictor_streams(B, steps + 70, tokens.device)
+        streams[1] = model.predictor_blocks[1].new_stream(B + (spoil == "batch"), 128 if spoil == "capacity" else 512, tokens.device)
+        taken = 0
+        while spoil == "capacity" and taken < steps:
+            model.predict_stream(tokens, streams)
+            taken += 1
+        with pytest.raises(ValueError):
+            model.predict_stream(tokens, streams)
+        assert streams[0].kv.lengths.tolist() == [taken * per] * B

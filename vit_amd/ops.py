@@ -462,6 +462,17 @@ class KVCache8:
         self.lengths.zero_()
         self.max_len = 0
 
+    def length_after(self, n: int, new: Optional[torch.Tensor] = None) -> int:
+        """The bound behind an append of n tokens (of stream b the first new[b]); raises where a stream would pass the capacity."""
+        after = self.max_len + n
+        if after > self.capacity:
+            # the bound counts padding: what the streams would really hold decides, where the device can be asked
+            if not torch.cuda.is_current_stream_capturing():
+                after = int((self.lengths + (n if new is None else new.clamp(0, n))).max())
+            if after > self.capacity:
+                raise ValueError(f"KVCache8: a stream would hold {after} tokens, the capacity is {self.capacity}")
+        return after
+
     def sync_length(self) -> int:
         """Set `max_len` to the longest stream's length, which the device is asked for (and waited for)."""
         if torch.cuda.is_current_stream_capturing():
@@ -501,13 +512,7 @@ def kv8_append_(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, new: Optional
     ldv, bsv = _token_strides(v, "v", (B, n, H, hd))
     if new is not None:
         _new_tokens(new, B)
-    after = cache.max_len + n
-    if after > cache.capacity:
-        # the bound counts padding: what the streams would really hold decides, where the device can be asked
-        if not torch.cuda.is_current_stream_capturing():
-            after = int((cache.lengths + (n if new is None else new.clamp(0, n))).max())
-        if after > cache.capacity:
-            raise ValueError(f"kv8_append_: a stream would hold {after} tokens, the capacity is {cache.capacity}")
+    after = cache.length_after(n, new)
     check(_lib.load().va_kv8_append(k.data_ptr(), v.data_ptr(), ldk, ldv, bsk, bsv, _p(new), n, *cache.pointers(), B, H, hd,
                                     cache.capacity, _stream()), "va_kv8_append")
     cache.max_len = after

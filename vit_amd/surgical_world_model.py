@@ -812,8 +812,13 @@ class SurgicalActionConditionedWorldModel(nn.Module):
         them -> the normalised predictor features of those tokens, as `forward` computes them for the whole sequence so
         far.  Each timestep costs its own tokens and one pass over the 8-bit cache instead of the whole sequence."""
         per_step = self.tokens_per_frame + 2
-        if len(streams) != len(self.predictor_blocks):       # before any of them has taken the tokens
+        # before any of them has taken the tokens
+        if len(streams) != len(self.predictor_blocks):
             raise ValueError(f"predict_stream: {len(streams)} states for {len(self.predictor_blocks)} predictor blocks")
+        for stream in streams:
+            if stream.kv.batch != tokens.shape[0]:
+                raise ValueError(f"predict_stream: {tokens.shape[0]} streams given, a state holds {stream.kv.batch}")
+            stream.kv.length_after(tokens.shape[1])
         for blk, stream in zip(self.predictor_blocks, streams):
             tokens = blk.stream(tokens, stream, per_step)
         return self.predictor_norm(tokens)
