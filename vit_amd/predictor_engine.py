@@ -37,7 +37,9 @@ def block_supported(blk, x: torch.Tensor) -> bool:
 def delta_rule(q, k, v, alpha, beta, state):
     """The memory layer's recurrence without a graph: token by token below 64 tokens (512 heads x 32 tokens of head dim 128:
     40 against 58 us; one stream of 8 heads: 22 against 22), chunks of 64 from there on (512 x 64: 61 against 65 us, 512 x 2064:
-    1.24 against 1.67 ms; 8 x 258: 47 against 151 us).  The two add the same f32 products in another order."""
+    1.24 against 1.67 ms; 8 x 258: 47 against 151 us).  The two add the same f32 products in another order.  A whole block over
+    the next tokens of 64 streams takes 316 against 356 us for 10 tokens, 572 against 581 for 60; of one stream 281 against 289
+    for 30, 303 against 295 for 60."""
     if q.shape[1] < 64:
         return ops.gated_delta_seq(q, k, v, alpha, beta, state)
     return ops.gated_delta_fwd(q, k, v, alpha, beta, state)
@@ -160,7 +162,7 @@ def _memory_stream(t, x_mid: torch.Tensor, B: int, n: int, stream: BlockStream, 
         # the three leading rows leave the state as it is: decay 1, nothing written
         a_ext = torch.cat([alpha.new_ones(B, 3, Hd), alpha.view(B, n, Hd)], dim=1)
         b_ext = torch.cat([beta.new_zeros(B, 3, Hd), beta.view(B, n, Hd)], dim=1)
-        out, state = ops.gated_delta_fwd(q, k, v, a_ext, b_ext, stream.state)
+        out, state = delta_rule(q, k, v, a_ext, b_ext, stream.state)
         stream.state.copy_(state)
         out = out[:, 3:]
     on = torch.empty(M, inner, dtype=BF16, device=dev)
