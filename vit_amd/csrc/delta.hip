@@ -25,8 +25,9 @@
 // Numbers on the matrix pipe.  The bf16 instruction (16x16x32) does sixteen times the products of the f32 one (16x16x4) per
 // cycle, so the scans split every f32 operand into three bf16 numbers, x = x0 + x1 + x2 with |x1| <= 2^-8 |x| and
 // |x2| <= 2^-16 |x| (nothing is left of 24 bits), and add the six products x_a y_b with a + b <= 2 into one f32 accumulator;
-// what is left out is below 2^-24 of |x y|, the rounding of an f32 product.  bf16 inputs are one such number: three products.
-// Where a result is rounded to bf16 in the end, two numbers per operand are kept (2^-16).  The 64x64 systems (prep) and the
+// what is left out, x1 y2 + x2 y1 + x2 y2, is at most 2^-23 + 2^-32 of |x y|, an f32 product's step.  bf16 inputs are one such
+// number: three products.  Where a result is rounded to bf16 in the end, two numbers per operand are kept: 2^-16 of each operand
+// and of each product is lost, a 256th of that rounding's half step.  The 64x64 systems (prep) and the
 // last gradients (grad) run on the f32 instruction.
 // Both instructions take a right operand from an accumulator as it lies: register r of lane group g holds row 4g+r of a tile,
 // and any order of the contraction index will do if the left operand follows it: for the f32 one index 4g+r at step r, for

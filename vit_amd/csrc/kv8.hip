@@ -4,7 +4,8 @@
 // full yet lies beside it in bf16 [64][hd], so what a block's codes are depends on its 64 tokens alone and not on how many
 // came in one call.  A scale is the smallest power of two (2^-100 at least) that brings the block's largest finite magnitude
 // to 448 or below: a code times its scale is then a bf16 number exactly, and the only rounding of a key or value is the one
-// to its code (half a step, 2^-4 of the value).  Infinite elements become NaN.
+// to its code, half a step: 2^-4 of the value at most, or 2^-10 of the scale for values below 2^-6 of it, where e4m3's steps no
+// longer shrink (elements under 2^-10 of the scale become zero).  Infinite elements become NaN.
 //
 // Attention: query row r of a key/value head = (query r / G, head r % G of its G query heads); query i of a stream with
 // `len` tokens of which `nb` are new stands at p = len - nb + i and sees keys j < limit: len, or with T tokens to a timestep

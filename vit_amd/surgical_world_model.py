@@ -389,7 +389,8 @@ class VideoViTEncoder(nn.Module):
 # predictor side.  Inference (no autograd graph, tensors on the device) runs the memory layer's causal
 # conv + SiLU (+ normalise), the delta-rule recurrence and the block-causal attention on the HIP kernels;
 # projections and the small heads are library GEMMs through torch.  With autograd the torch formulation of
-# the same arithmetic is used (the predictor is not trained by the stage-1 scripts).
+# the same arithmetic is used (the predictor is not trained by the stage-1 scripts), around the kernels of the
+# memory layer's recurrence and output stage, which have gradients.
 # =====================================================================================================
 def _hip_inference(x: torch.Tensor, module: Optional[nn.Module] = None) -> bool:
     """True when the inference kernels may run: device f32 input and no autograd graph to build -- neither through
@@ -417,9 +418,10 @@ def _note_torch_path(x: torch.Tensor, who: str) -> None:
     _warned_torch_path = True
     import warnings
     warnings.warn(f"{who}: grad mode is on and the predictor has trainable parameters (or its input requires grad), so "
-                  "this call is computed by the torch formulation, with the memory layer's recurrence and output stage on "
-                  "their differentiable HIP kernels (head dims 64 and 128). For inference wrap the call in "
-                  "torch.no_grad().", RuntimeWarning, stacklevel=3)
+                  "this call is computed by the torch formulation. Only the memory layer's recurrence and output stage have "
+                  "HIP kernels with gradients (f32, head dims 64 and 128; torch too under torch.func, forward-mode "
+                  "derivatives, autocast and tracing). For inference wrap the call in torch.no_grad().", RuntimeWarning,
+                  stacklevel=3)
 
 
 def _as_torch_made_it(module: nn.Module, kind) -> bool:
