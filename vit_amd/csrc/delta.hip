@@ -229,7 +229,7 @@ VA_DEVINL void row_frag(const char* x, int it, int u, int m, int g, bf16x8_t (&o
 // row i and four consecutive j; the wave with row tile w of K K^T (w + 1 tiles) takes row tile 3 - w of Q K^T, five tiles to
 // each.  Writes T and P; TRAIN: T^T and P^T as well, for the gradient's scan (P^T's tiles are formed the other way round).
 // Bound by memory when there are many chunks (100 KB of f32 rows and operands per chunk: 16 896 chunks of head dim 128 in
-// 480 us, 3.5 TB/s), by its chain of small systems when there are few (40 chunks of bf16 rows: 9.9 us).  bf16 rows stay bf16
+// 408 us, 4.1 TB/s), by its chain of small systems when there are few (40 chunks of bf16 rows: 9.6 us).  bf16 rows stay bf16
 // in LDS and are multiplied by the bf16 instruction, whose products of them are exact (with f32 copies and the f32 instruction
 // the 40 chunks took 12 us).  A and T lie over K in LDS so that three workgroups share a CU.
 template <int HD, typename T, bool TRAIN>
@@ -592,7 +592,7 @@ VA_DEVINL void rows_by_token(const T* q, const T* k, const T* v, int64_t ldq, in
 // OUT: writes o.  SAVE: writes U and every chunk's starting state (rows of S) for the gradient.
 // Bound by its chain: per chunk and wave 360 matrix instructions (f32, head dim 128; 182 for bf16), about as many cycles of
 // vector work (splits, addresses) and of LDS reads, which one wave per SIMD runs one after the other: 7.7 us a chunk for f32, 5
-// for bf16; 512 heads x 2064 tokens of f32 in 0.8-0.95 ms (2.2 GB and 0.6 GB of operands).
+// for bf16; 512 heads x 2064 tokens of f32 in 0.81 ms (2.2 GB and 0.6 GB of operands).
 // A product with a zero does not silence a NaN, and an infinity has no parts: a token with either would reach earlier tokens of
 // its chunk.  A wave that ends with a non-finite output or state forms its rows again token by token, so that what the
 // recurrence leaves finite is finite; the outputs of the chunks before stay.
@@ -760,7 +760,7 @@ __global__ __launch_bounds__(64 * W) void delta_scan_kernel(const T* __restrict_
 
 // ---------------------------------------------------------------------------------------------------------------
 // The same walk backwards for G = dL/dM: writes every chunk's G (at its end, rows of dS), R and dv.  Bound as the scan: 32 heads
-// x 21 chunks of f32, head dim 128, in 168 us.
+// x 21 chunks of f32, head dim 128, in 167 us.
 template <int HD, typename T, int W, int CG>
 __global__ __launch_bounds__(64 * W) void delta_rscan_kernel(const T* __restrict__ Q, const T* __restrict__ K, Rows rq, Rows rk,
                                                              const T* __restrict__ DO, const float* __restrict__ BETA,
@@ -893,7 +893,7 @@ template <int HD> struct GradLds {                 // byte offsets
 // half of the rows of dQ and dK (a chunk's M and G are read twice, its other operands four times; with an eighth of the columns
 // and all rows it was 177 instead of 152 us at 672 chunks of f32, head dim 128; four waves 154).  The 64x64 matrices are formed tile by tile
 // and shared through LDS.  Bound by the f32 matrix instruction (6000 per chunk, a third of the time) and the waits between its
-// phases: 672 chunks of f32, head dim 128, in 152 us, 432 of bf16, head dim 64, in 52.
+// phases: 672 chunks of f32, head dim 128, in 147 us, 432 of bf16, head dim 64, in 52.
 template <int HD, typename T>
 __global__ __launch_bounds__(512) void delta_grad_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                                                          Rows rq, Rows rk, Rows rv, const T* __restrict__ DO,
@@ -1194,7 +1194,7 @@ template <> struct elem<bf16_t> {
 //     dk = G^T u - a b P^T (G k),     G <- a (G - b (G k) k^T).
 // P is formed anew from the chunk's first state for each token (GS, whose chunked contents are of no use, holds those): rare, so
 // this trades time for memory (32 heads x 1290 tokens of f32, head dim 128, all bad: 37 ms).  Heads whose results are finite
-// leave at once.
+// leave at once (a launch of 4-5 us behind the others).
 template <int HD, typename T>
 __global__ __launch_bounds__(4 * HD) void delta_grad_by_token_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                                      const T* __restrict__ V, Rows rq, Rows rk, Rows rv,
@@ -1320,7 +1320,8 @@ __global__ __launch_bounds__(4 * HD) void delta_grad_by_token_kernel(const T* __
 // ---------------------------------------------------------------------------------------------------------------
 // One token: S <- a S + u k^T, u = b (v - a S k), o = S q = a (S_old q) + u (k.q).  The state is read and written once and
 // its rows are independent: HD/4 lanes hold a row (16 bytes each), the row's two dot products are summed across them.  Bound by
-// the state's bytes: 2048 heads of 128 in 44 us, 6.1 TB/s; 8 heads in 3 us.
+// the state's bytes: 2048 heads of 128 in 57 us, 4.8 TB/s (44 where the last-level cache still holds the states);
+// 8 heads in 3 us.
 template <int HD, typename T>
 __global__ __launch_bounds__(256) void delta_step_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                                                          int64_t ldq, int64_t ldk, int64_t ldv, const float* __restrict__ ALPHA,

@@ -33,7 +33,8 @@ struct Cache {
 // ---- append ---------------------------------------------------------------------------------------------------
 // One workgroup per block that the call touches, head and stream, keys or values.  Where the open block fills up and a
 // later one is left open, one workgroup does both: it has read the open block before it writes the new one over it.  Bound by
-// launches for single tokens (below 4 us), by memory for long calls (16 streams x 1290 tokens x 8 heads of 128: 23 us, 5.5 TB/s).
+// launches for single tokens (3 us, 5 where a block fills up), by memory for long calls (16 streams x 1290 tokens x 8 heads of
+// 128: 28 us, 4.6 TB/s; 258 tokens behind them 11 us).
 template <int HD>
 __global__ __launch_bounds__(256) void kv8_append_kernel(const bf16_t* __restrict__ K, const bf16_t* __restrict__ V, int64_t ldk,
                                                          int64_t ldv, int64_t bsk, int64_t bsv, const int32_t* __restrict__ NEW,
@@ -281,7 +282,7 @@ VA_DEVINL void tile_pv(const char* vt, int stride, const bf16x8_t (&pf)[2], f32x
 // Few rows (up to 16 per key/value head): bound by the cache's bytes.  Waves take tiles in turn, each with its own running
 // state; keys go straight from memory to operands, values through a private piece of LDS for their transposition, the next
 // tile's bytes are requested before the current one is used.  Streams and heads that leave CUs idle are split over the keys.
-// 32 streams of up to 8256 tokens, 8 heads of 128 with four query heads each: 92 us, 4.4 TB/s (two workgroups to a CU; with
+// 32 streams of up to 8256 tokens, 8 heads of 128 with four query heads each: 91 us, 4.5 TB/s (two workgroups to a CU; with
 // one 105, with four 100).
 template <int HD>
 __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(Cache c, AttnArgs a) {
